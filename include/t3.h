@@ -312,6 +312,60 @@ typedef struct t3_engines {
 void t3_engines_held(t3_engines* out);
 void t3_release_engines(void);
 
+/* ---- 8-bit layers and routing -------------------------------------------------------------------------------------------
+ * What a checkpoint keeps in 8-bit floating point beside its EXL3 layers (e4m3 values, one f32 scale for each block of 128), and
+ * the routing ahead of a routed layer of either kind. No counterpart in the reference, which leaves both to its host. The same
+ * rules as above: device pointers, caller-allocated outputs and scratch, every refusal before any launch, no synchronising,
+ * safe under stream capture. Pointers to activations, e4m3 values and outputs of linears start on 16 bytes, else BadExl3Shape. */
+#define T3_E4M3 3  /* a dtype of x in t3_linear_fp8 only */
+
+/* A router's choice: logits [rows, experts] in dtype -> inds i32 [rows, topk] and scores f32 [rows, topk], best first, the lower
+ * number first among equals: what t3_moe and t3_moe_fp8 take. scoring: softmax over the row's experts, or sigmoid. The largest logits are chosen;
+ * with `bias` (f32 [experts], or null) or groups > 1 the largest picks, pick = score + bias in 64 bits (the scores returned are
+ * without it). groups > 1: the experts are cut into `groups` equal runs, and only the group_topk runs with the largest sums of
+ * their two largest picks are chosen from (the lower run first among equals). renormalise: the chosen scores are divided by their
+ * sum (zeros where that is 0); then all are multiplied by `scale`. A logit at or below its type's lowest finite number removes its expert: it
+ * counts in no sum, is chosen only where too few others are left, and then has score 0 (a row with nothing left: all scores 0). A NaN
+ * logit ranks first and shows in the scores. experts 1..1024, topk 1..32 and no more than can be chosen from, groups 1..32 and a divisor of
+ * experts, group_topk 1..groups (1 with one group), scale finite, else BadExl3Shape. */
+typedef enum { T3_SCORE_SOFTMAX = 0, T3_SCORE_SIGMOID = 1 } t3_scoring;
+#define T3_ROUTE_EXPERTS_MAX 1024
+int t3_route(const void* logits, int dtype, size_t rows, int experts, int topk, int scoring, const void* bias, int groups, int group_topk,
+             int renormalise, float scale, void* inds, void* scores, void* stream);
+
+/* x [rows, in] (in a multiple of 128) -> q e4m3 [rows, in] and scale f32 [rows, in / 128]: a group of 128's scale is the smallest power of
+ * two, from 2^-126 up, that brings its largest magnitude to 448 or less; q = e4m3(x / scale), to nearest even. A group with an
+ * infinity or a NaN has a NaN as its scale and NaN values. */
+int t3_quantize_fp8(const void* x, int x_dtype, size_t rows, int in_dim, void* q, void* scale, void* stream);
+
+/* y [rows, out] in y_dtype = x W^T with W e4m3 [out, in], w_scale f32 [ceil(out / 128), in / 128]: in a multiple of 128, out any. x
+ * f32, f16 or bf16 is quantised as t3_quantize_fp8 does it (x_scale null); x_dtype T3_E4M3: x is q, x_scale its scales (any f32 values).
+ * Products and sums in f32, one rounding into y. The workspace (256-byte aligned) holds the quantised rows where the kernel does not
+ * quantise them itself: t3_linear_fp8_workspace_bytes, 0 for T3_E4M3. */
+size_t t3_linear_fp8_workspace_bytes(size_t rows, int in_dim, int out_dim, int x_dtype);
+int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, const void* w, const void* w_scale, int in_dim, int out_dim,
+                  void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A routed SwiGLU layer for a few tokens, its experts in e4m3: y[row] = sum over the row's slots of score * down(silu(gate x) * up x)
+ * (+ shared), in two launches. x [rows, hidden] is quantised as above, and so is silu(gate) * up (held in f32 until then). w: gate
+ * and up [experts, inter, hidden], down [experts, hidden, inter]; scales f32 [experts, out / 128, in / 128]; hidden and inter multiples of
+ * 128, experts 1..T3_FP8_EXPERTS_MAX. inds i32 / u32 and scores (scores_dtype) [rows, topk], topk 1..32; an id outside the bank is nobody's and
+ * adds nothing, whatever its score (a padded row's, or another rank's of an expert-parallel layer); an id may come twice. shared:
+ * [rows, hidden] in x's dtype added before the one rounding, or null. y in x's dtype. Rows 1..T3_DECODE_ROWS_MAX, more:
+ * Exl3EngineNotImplemented. Workspace (256-byte aligned): t3_moe_fp8_workspace_bytes. */
+#define T3_FP8_EXPERTS_MAX 2048
+typedef struct {
+    const void* w;
+    const void* scale;
+} t3_fp8_proj;
+typedef struct {
+    t3_fp8_proj gate, up, down;
+    int experts, hidden, inter;
+} t3_fp8_bank;
+size_t t3_moe_fp8_workspace_bytes(size_t rows, int topk, const t3_fp8_bank* bank);
+int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank, const void* inds, const void* scores, int scores_dtype,
+               int topk, const void* shared, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Kernels this library launched since the process started (for benches that must report their launch count). */
 uint64_t t3_launch_count(void);
 

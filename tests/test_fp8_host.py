@@ -1,0 +1,120 @@
+"""CPU-only checks of the 8-bit layers' and the router's entry points: every refusal by its name, before the device is touched, and the
+workspaces' sizes."""
+import ctypes as C
+
+import pytest
+import torch
+
+import turboexl3_b200 as t3
+from turboexl3_b200 import api
+
+FAKE = 0x1000  # non-null and 256-byte aligned; a refusal never dereferences it
+
+
+def name(status):
+    return t3.status_name(status)
+
+
+def _route(logits=FAKE, dtype=0, rows=1, experts=64, topk=4, scoring=0, bias=None, groups=1, group_topk=1, scale=1.0, inds=FAKE, scores=FAKE):
+    return name(t3.lib().t3_route(logits, dtype, rows, experts, topk, scoring, bias, groups, group_topk, 1, scale, inds, scores, None))
+
+
+def test_route_refusals():
+    assert _route(logits=None) == "NullPointer"
+    assert _route(inds=None) == "NullPointer"
+    assert _route(scores=None) == "NullPointer"
+    assert _route(dtype=3) == "BadExl3Dtype"
+    assert _route(scoring=2) == "Exl3EngineNotImplemented"
+    for bad in (dict(rows=0), dict(experts=0), dict(experts=1025), dict(topk=0), dict(topk=33), dict(experts=3, topk=4), dict(groups=0),
+                dict(groups=33, experts=66), dict(groups=5), dict(groups=8, group_topk=9), dict(groups=8, group_topk=0),
+                dict(groups=32, group_topk=1, topk=3), dict(group_topk=2), dict(scale=float("nan")), dict(scale=float("inf"))):
+        assert _route(**bad) == "BadExl3Shape", bad
+
+
+def _quantize(x=FAKE, dt=2, rows=1, width=256, q=FAKE, scale=FAKE):
+    return name(t3.lib().t3_quantize_fp8(x, dt, rows, width, q, scale, None))
+
+
+def test_quantize_refusals():
+    for bad in (dict(x=None), dict(q=None), dict(scale=None)):
+        assert _quantize(**bad) == "NullPointer"
+    assert _quantize(dt=3) == "BadExl3Dtype"
+    for bad in (dict(rows=0), dict(width=0), dict(width=200), dict(width=-128), dict(x=FAKE + 8), dict(q=FAKE + 8)):
+        assert _quantize(**bad) == "BadExl3Shape", bad
+
+
+def _linear(x=FAKE, dt=2, xs=None, rows=1, w=FAKE, ws=FAKE, width=256, out=256, y=FAKE, ydt=2, work=FAKE, work_bytes=1 << 40):
+    return name(t3.lib().t3_linear_fp8(x, dt, xs, rows, w, ws, width, out, y, ydt, work, work_bytes, None))
+
+
+def test_linear_refusals():
+    for bad in (dict(x=None), dict(w=None), dict(ws=None), dict(y=None), dict(dt=3, xs=None)):
+        assert _linear(**bad) == "NullPointer", bad
+    for bad in (dict(dt=4), dict(dt=-1), dict(ydt=3)):
+        assert _linear(**bad) == "BadExl3Dtype", bad
+    for bad in (dict(rows=0), dict(width=0), dict(width=200), dict(out=0), dict(out=-1), dict(xs=FAKE), dict(x=FAKE + 4), dict(w=FAKE + 8),
+                dict(y=FAKE + 2), dict(rows=1 << 23, width=1024)):
+        assert _linear(**bad) == "BadExl3Shape", bad
+    assert _linear(rows=200, work=None) == "NullPointer"
+    assert _linear(rows=200, work_bytes=16) == "WorkspaceTooSmall"
+    assert _linear(rows=200, work=FAKE + 16) == "WorkspaceTooSmall"
+
+
+def test_linear_past_decode_rows_follows_the_configuration():
+    t3.configure(prefill=False)
+    try:
+        assert _linear(rows=33) == "Exl3EngineNotImplemented"
+    finally:
+        t3.configure()
+
+
+def test_linear_workspace():
+    L = t3.lib()
+    assert L.t3_linear_fp8_workspace_bytes(1, 2048, 2048, 2) == 0            # the kernel quantises the row itself
+    assert L.t3_linear_fp8_workspace_bytes(200, 2048, 2048, api.E4M3) == 0   # quantised already
+    assert L.t3_linear_fp8_workspace_bytes(200, 2048, 2048, 2) >= 200 * (2048 + 16 * 4)
+    assert L.t3_linear_fp8_workspace_bytes(0, 2048, 2048, 2) == 0
+
+
+def _bank(experts=8, hidden=256, inter=128, **null):
+    p = [api._Fp8Proj(null.get("w", FAKE), null.get("scale", FAKE)) for _ in range(3)]
+    return api._Fp8Bank(*p, experts, hidden, inter)
+
+
+def _moe(bank=None, x=FAKE, dt=2, rows=1, inds=FAKE, scores=FAKE, sdt=0, topk=2, shared=None, y=FAKE, work=FAKE, work_bytes=1 << 40):
+    b = bank or _bank()
+    return name(t3.lib().t3_moe_fp8(x, dt, rows, C.byref(b), inds, scores, sdt, topk, shared, y, work, work_bytes, None))
+
+
+def test_moe_refusals():
+    for bad in (dict(x=None), dict(inds=None), dict(scores=None), dict(y=None), dict(work=None), dict(bank=_bank(w=None)),
+                dict(bank=_bank(scale=None))):
+        assert _moe(**bad) == "NullPointer", bad
+    for bad in (dict(dt=3), dict(sdt=3)):
+        assert _moe(**bad) == "BadExl3Dtype", bad
+    for bad in (dict(bank=_bank(hidden=200)), dict(bank=_bank(inter=64)), dict(bank=_bank(experts=0)), dict(bank=_bank(experts=2049)),
+                dict(bank=_bank(experts=2048, hidden=1 << 20)), dict(rows=0), dict(topk=0), dict(topk=33), dict(x=FAKE + 8),
+                dict(bank=_bank(w=FAKE + 8))):
+        assert _moe(**bad) == "BadExl3Shape", bad
+    assert _moe(rows=33) == "Exl3EngineNotImplemented"
+    assert _moe(work_bytes=16) == "WorkspaceTooSmall"
+    assert _moe(work=FAKE + 16) == "WorkspaceTooSmall"
+
+
+@pytest.mark.parametrize("rows,topk,experts,hidden,inter", [(1, 1, 1, 128, 128), (32, 32, 2048, 7168, 2048), (32, 10, 512, 2048, 512), (17, 8, 64, 16384, 4096)])
+def test_moe_workspace_covers_the_experts_in_use(rows, topk, experts, hidden, inter):
+    b = _bank(experts, hidden, inter)
+    used, cap = min(experts, rows * topk), 16 if rows <= 16 else 32
+    assert t3.lib().t3_moe_fp8_workspace_bytes(rows, topk, C.byref(b)) >= used * cap * (inter + inter // 128 * 4)
+
+
+def test_python_refusals():
+    x, logits = torch.zeros(2, 256), torch.zeros(2, 64)
+    w, s = torch.zeros(256, 256).to(torch.float8_e4m3fn), torch.ones(2, 2)
+    for call in (lambda: t3.route(logits, 4), lambda: t3.quantize_fp8(x), lambda: t3.linear_fp8(x, w, s)):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
+    with pytest.raises(t3.Exl3Error, match="Exl3EngineNotImplemented"):
+        t3.route(logits, 4, "tanh")
+    with pytest.raises(t3.Exl3Error, match="BadExl3Dtype"):
+        t3.linear_fp8(x, w, s, out_dtype=torch.int8)

@@ -52,6 +52,14 @@ class _Spec(C.Structure):
     _fields_ = [("n", C.c_uint32), ("codebook", C.c_int), ("window_bits", C.c_int)]
 
 
+class _Fp8Proj(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("scale", C.c_void_p)]
+
+
+class _Fp8Bank(C.Structure):
+    _fields_ = [("gate", _Fp8Proj), ("up", _Fp8Proj), ("down", _Fp8Proj), ("experts", C.c_int), ("hidden", C.c_int), ("inter", C.c_int)]
+
+
 class Launch(C.Structure):
     """t3_launch: one kernel launch of a plan (symbol, group, grid, block, shared bytes, cluster size, buffer roles)."""
     _fields_ = [("symbol", C.c_char * 64), ("group", C.c_char * 16), ("grid", C.c_uint32 * 3), ("block", C.c_uint32),
@@ -103,6 +111,12 @@ SYMBOLS = {
     "t3_plan_linear": (_i, [_sz, _i, _i, _i, _Decode, C.POINTER(Launch), _i]),
     "t3_plan_moe": (_i, [_sz, _i, C.POINTER(_Bank), _Decode, C.POINTER(Launch), _i]),
     "t3_last_kernel_symbol": (C.c_char_p, []),
+    "t3_route": (_i, [_vp, _i, _sz, _i, _i, _i, _vp, _i, _i, _i, C.c_float, _vp, _vp, _vp]),
+    "t3_quantize_fp8": (_i, [_vp, _i, _sz, _i, _vp, _vp, _vp]),
+    "t3_linear_fp8_workspace_bytes": (_sz, [_sz, _i, _i, _i]),
+    "t3_linear_fp8": (_i, [_vp, _i, _vp, _sz, _vp, _vp, _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "t3_moe_fp8_workspace_bytes": (_sz, [_sz, _i, C.POINTER(_Fp8Bank)]),
+    "t3_moe_fp8": (_i, [_vp, _i, _sz, C.POINTER(_Fp8Bank), _vp, _vp, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     "t3_engines_held": (None, [_vp]),
     "t3_release_engines": (None, []),
 }
@@ -575,3 +589,117 @@ def moe_with_shared(x, bank: Bank, inds, scores, dec: Decode, shared: torch.Tens
     if shared is None or (shared_ready is not None and not shared_ready.cuda_event):  # an event nobody has recorded has no handle
         raise Exl3Error(14, "NullPointer")
     return _moe(x, bank, inds, scores, dec, 0, CLAMP_GATE_IN, shared, shared_ready=shared_ready)
+
+
+# ---- 8-bit layers and routing ------------------------------------------------------------------------------------------
+
+E4M3 = 3  # T3_E4M3: a dtype of x in t3_linear_fp8 only
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+ROUTE_EXPERTS_MAX = 1024
+FP8_EXPERTS_MAX = 2048
+
+
+@dataclass
+class Fp8Proj:
+    """A projection of an 8-bit bank: w float8_e4m3fn [E, out, in], scale f32 [E, out/128, in/128], one for each 128 x 128 block."""
+    w: torch.Tensor
+    scale: torch.Tensor
+
+
+@dataclass
+class Fp8Bank:
+    """A routed bank in 8 bits: gate and up [E, inter, hidden], down [E, hidden, inter]."""
+    gate: Fp8Proj
+    up: Fp8Proj
+    down: Fp8Proj
+
+
+def route(logits: torch.Tensor, topk: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+          group_topk: int = 1, renormalise: bool = True, scale: float = 1.0):
+    """A router's choice (t3_route): logits [..., experts] -> (inds int32 [..., topk], scores f32 [..., topk]), best first, as `moe` and
+    `moe_fp8` take them. The largest logits, the lower number among equals; with `bias` (f32 [experts]) or `groups` > 1 the largest
+    score + bias, out of the `group_topk` groups with the largest sums of two. A logit at or below its type's lowest finite
+    number removes its expert; a row with nothing left has scores of 0."""
+    if scoring not in SCORINGS:
+        raise Exl3Error(3, "Exl3EngineNotImplemented")
+    y = (_call or native()).route(logits, topk, SCORINGS[scoring], bias, groups, group_topk, renormalise, scale)
+    return y if y.__class__ is tuple else _refuse_route(y, logits, topk, bias)
+
+
+def _refuse_route(status, logits, topk, bias):
+    if status is not None:
+        _check(status)
+    _need_cuda(logits)
+    if bias is not None:
+        _need_cuda(bias)
+        if bias.dtype != torch.float32:
+            raise Exl3Error(2, "BadExl3Dtype")
+    if logits.dtype not in _DTYPES:
+        raise Exl3Error(2, "BadExl3Dtype")
+    raise Exl3Error(1, "BadExl3Shape")
+
+
+def quantize_fp8(x: torch.Tensor):
+    """x [..., in] to e4m3 (t3_quantize_fp8): (q float8_e4m3fn [..., in], scale f32 [..., in/128]), one power-of-two scale for each 128
+    values of a row."""
+    y = (_call or native()).quantize_fp8(x)
+    return y if y.__class__ is tuple else _refuse_quantize_fp8(y, x)
+
+
+def _refuse_quantize_fp8(status, x):
+    if status is not None:
+        _check(status)
+    _need_cuda(x)
+    if x.dtype not in _DTYPES:
+        raise Exl3Error(2, "BadExl3Dtype")
+    raise Exl3Error(1, "BadExl3Shape")
+
+
+def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y [..., out] = x W^T with W float8_e4m3fn [out, in] and w_scale f32 [ceil(out/128), in/128] (t3_linear_fp8). x [..., in] in f32,
+    f16 or bf16, quantised as `quantize_fp8` does it, or its (q, scale) as x and x_scale. out_dtype: x's, bf16 for a quantised x."""
+    if out_dtype is not None and out_dtype not in _DTYPES:
+        raise Exl3Error(2, "BadExl3Dtype")
+    y = (_call or native()).linear_fp8(x, w, w_scale, x_scale, -1 if out_dtype is None else _DTYPES[out_dtype])
+    return y if y.__class__ is torch.Tensor else _refuse_linear_fp8(y, x, w, w_scale, x_scale)
+
+
+def _refuse_linear_fp8(status, x, w, w_scale, x_scale):
+    if status is not None:
+        _check(status)
+    _need_cuda(x, w, w_scale)
+    if x_scale is not None:
+        _need_cuda(x_scale)
+    given = x.dtype == torch.float8_e4m3fn
+    if (x.dtype not in _DTYPES and not given) or w.dtype != torch.float8_e4m3fn or w_scale.dtype != torch.float32:
+        raise Exl3Error(2, "BadExl3Dtype")
+    if given and x_scale is None:
+        raise Exl3Error(14, "NullPointer")
+    if given and x_scale.dtype != torch.float32:
+        raise Exl3Error(2, "BadExl3Dtype")
+    raise Exl3Error(1, "BadExl3Shape")
+
+
+def moe_fp8(x: torch.Tensor, bank: Fp8Bank, inds: torch.Tensor, scores: torch.Tensor, shared: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A routed SwiGLU layer in 8 bits for a few tokens (t3_moe_fp8): x [B, S, D] with B * S up to DECODE_ROWS_MAX, inds / scores
+    [B, S, K]; y in x's shape and dtype. An id outside the bank adds nothing. shared: [B, S, D], added before the one rounding."""
+    y = (_call or native()).moe_fp8(x, bank, inds, scores, shared)
+    return y if y.__class__ is torch.Tensor else _refuse_moe_fp8(y, x, bank, inds, scores, shared)
+
+
+def _refuse_moe_fp8(status, x, bank, inds, scores, shared):
+    if status is not None:
+        _check(status)
+    _need_cuda(x, inds, scores)
+    if x.dim() != 3 or inds.dim() != 3 or x.shape[:2] != inds.shape[:2] or inds.shape != scores.shape:
+        raise Exl3Error(1, "BadExl3Shape")
+    if x.dtype not in _DTYPES or inds.dtype not in (torch.int32, torch.uint32) or scores.dtype not in _DTYPES:
+        raise Exl3Error(2, "BadExl3Dtype")
+    for p in (bank.gate, bank.up, bank.down):
+        _need_cuda(p.w, p.scale)
+        if p.w.dtype != torch.float8_e4m3fn or p.scale.dtype != torch.float32:
+            raise Exl3Error(2, "BadExl3Dtype")
+    if shared is not None:
+        _need_cuda(shared)
+    raise Exl3Error(1, "BadExl3Shape")

@@ -29,6 +29,10 @@ UNITS = [
     ("t3_gemm.cu", "t3_gemm_cb0", ["-DT3_CB=0"]),
     ("t3_gemm.cu", "t3_gemm_cb1", ["-DT3_CB=1"]),
     ("t3_api.cu", "t3_api", []),
+    ("t3_fp8_api.cu", "t3_fp8_api", []),
+    ("t3_fp8_rows.cu", "t3_fp8_rows", []),
+    ("t3_fp8_quant.cu", "t3_fp8_quant", []),
+    ("t3_route.cu", "t3_route", []),
     ("t3_dequant.cu", "t3_dequant", []),
     ("t3_decode_rows.cu", "t3_decode_rows_cb0", ["-DT3_CB=0"]),
     ("t3_decode_rows.cu", "t3_decode_rows_cb1", ["-DT3_CB=1"]),

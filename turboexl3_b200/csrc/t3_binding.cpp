@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -17,7 +18,7 @@
 
 namespace {
 
-PyObject *s_trellis, *s_suh, *s_svh, *s_gate, *s_up, *s_down, *s_codebook, *s_window_bits;
+PyObject *s_trellis, *s_suh, *s_svh, *s_gate, *s_up, *s_down, *s_codebook, *s_window_bits, *s_w, *s_scale;
 
 // an attribute whose holder keeps it alive (instances of the package's dataclasses)
 struct Attr {
@@ -162,6 +163,162 @@ PyObject* call_moe(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit layers and routing: every tensor on x's device, which need not be the current one ----
+
+bool is_e4m3(const at::Tensor& t) { return t.scalar_type() == at::kFloat8_e4m3fn; }
+bool is_f32(const at::Tensor& t) { return t.scalar_type() == at::kFloat; }
+
+// route(logits, topk, scoring, bias or None, groups, group_topk, renormalise, scale)
+PyObject* call_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 8) Py_RETURN_NONE;
+    const at::Tensor *x = tensor(args[0]), *bias = nullptr;
+    if (!x || x->dim() < 1 || act_dtype(*x) < 0) Py_RETURN_NONE;
+    const int64_t experts = x->size(-1);
+    if (args[3] != Py_None) {
+        bias = tensor(args[3]);
+        if (!bias || !is_f32(*bias) || bias->numel() != experts || bias->device() != x->device()) Py_RETURN_NONE;
+    }
+    const long topk = PyLong_AsLong(args[1]), scoring = PyLong_AsLong(args[2]), groups = PyLong_AsLong(args[4]),
+               group_topk = PyLong_AsLong(args[5]), renormalise = PyObject_IsTrue(args[6]);
+    const double scale = PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (experts < 1 || experts > T3_ROUTE_EXPERTS_MAX || x->numel() < 1 || topk < 1 || topk > T3_REDUCE_MAX_TOPK || groups < 1 || groups > 32 ||
+        group_topk < 1 || group_topk > 32)
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(x->device());
+    c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = topk;
+    at::Tensor inds = empty(shape, at::kInt, *x), scores = empty(shape, at::kFloat, *x);
+    void* stream = stream_of(*x);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = t3_route(x->data_ptr(), act_dtype(*x), (size_t)(x->numel() / experts), (int)experts, (int)topk, (int)scoring,
+                      bias ? bias->data_ptr() : nullptr, (int)groups, (int)group_topk, (int)renormalise, (float)scale, inds.data_ptr(),
+                      scores.data_ptr(), stream);
+    Py_END_ALLOW_THREADS
+    if (status != T3_OK) return PyLong_FromLong(status);
+    PyObject* i = THPVariable_Wrap(std::move(inds));
+    PyObject* s = THPVariable_Wrap(std::move(scores));
+    return Py_BuildValue("(NN)", i, s);
+    END_HANDLE_TH_ERRORS
+}
+
+// quantize_fp8(x)
+PyObject* call_quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 1) Py_RETURN_NONE;
+    const at::Tensor* x = tensor(args[0]);
+    if (!x || x->dim() < 1 || act_dtype(*x) < 0 || x->numel() < 1 || x->size(-1) % 128 != 0 || x->size(-1) > INT32_MAX) Py_RETURN_NONE;
+    const int64_t in = x->size(-1);
+    const c10::cuda::CUDAGuard guard(x->device());
+    c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
+    at::Tensor q = empty(shape, at::kFloat8_e4m3fn, *x);
+    shape.back() = in / 128;
+    at::Tensor scale = empty(shape, at::kFloat, *x);
+    void* stream = stream_of(*x);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = t3_quantize_fp8(x->data_ptr(), act_dtype(*x), (size_t)(x->numel() / in), (int)in, q.data_ptr(), scale.data_ptr(), stream);
+    Py_END_ALLOW_THREADS
+    if (status != T3_OK) return PyLong_FromLong(status);
+    PyObject* a = THPVariable_Wrap(std::move(q));
+    PyObject* b = THPVariable_Wrap(std::move(scale));
+    return Py_BuildValue("(NN)", a, b);
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_fp8(x, w, w_scale, x_scale or None, out_dtype: a t3_dtype, or -1 for x's)
+PyObject* call_linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 5) Py_RETURN_NONE;
+    const at::Tensor *x = tensor(args[0]), *w = tensor(args[1]), *ws = tensor(args[2]), *xs = nullptr;
+    if (!x || !w || !ws || x->dim() < 1 || w->dim() != 2 || ws->dim() != 2 || !is_e4m3(*w) || !is_f32(*ws)) Py_RETURN_NONE;
+    const int64_t in = w->size(1), out = w->size(0);
+    const bool given = is_e4m3(*x);
+    int dt = given ? T3_E4M3 : act_dtype(*x), ydt = (int)PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (ydt < 0) ydt = given ? T3_BF16 : dt;
+    if (dt < 0 || ydt > T3_BF16 || in < 1 || in > INT32_MAX || out < 1 || out > INT32_MAX || in % 128 != 0 || x->size(-1) != in || x->numel() < 1 ||
+        ws->size(0) != (out + 127) / 128 || ws->size(1) != in / 128 || w->device() != x->device() || ws->device() != x->device())
+        Py_RETURN_NONE;
+    if ((args[3] != Py_None) != given) Py_RETURN_NONE;
+    if (given) {
+        xs = tensor(args[3]);
+        if (!xs || !is_f32(*xs) || xs->numel() != x->numel() / 128 || xs->dim() != x->dim() || xs->size(-1) != in / 128 ||
+            xs->device() != x->device())
+            Py_RETURN_NONE;
+    }
+    const int64_t rows = x->numel() / in;
+    const c10::cuda::CUDAGuard guard(x->device());
+    c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = out;
+    at::Tensor y = empty(shape, ydt == T3_F32 ? at::kFloat : ydt == T3_F16 ? at::kHalf : at::kBFloat16, *x), scratch;
+    const size_t bytes = given ? 0 : t3_linear_fp8_workspace_bytes((size_t)rows, (int)in, (int)out, dt);
+    if (bytes) scratch = empty({(int64_t)bytes}, at::kByte, *x);
+    void* stream = stream_of(*x);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = t3_linear_fp8(x->data_ptr(), dt, xs ? xs->data_ptr() : nullptr, (size_t)rows, w->data_ptr(), ws->data_ptr(), (int)in, (int)out,
+                           y.data_ptr(), ydt, bytes ? scratch.data_ptr() : nullptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(status, y);
+    END_HANDLE_TH_ERRORS
+}
+
+// One projection of an 8-bit bank: w e4m3 [E, out, in], scale f32 [E, out / 128, in / 128]
+bool fp8_proj_of(PyObject* bank, PyObject* name, const at::Device& device, t3_fp8_proj& p, int64_t (&dims)[3]) {
+    Attr proj(bank, name);
+    if (!proj.p) return false;
+    Attr wo(proj.p, s_w), so(proj.p, s_scale);
+    if (!wo.p || !so.p) return false;
+    const at::Tensor *w = tensor(wo.p), *s = tensor(so.p);
+    if (!w || !s || w->dim() != 3 || s->dim() != 3 || !is_e4m3(*w) || !is_f32(*s) || w->device() != device || s->device() != device) return false;
+    for (int i = 0; i < 3; ++i) dims[i] = w->size(i);
+    if (dims[1] % 128 != 0 || dims[2] % 128 != 0 || s->size(0) != dims[0] || s->size(1) != dims[1] / 128 || s->size(2) != dims[2] / 128) return false;
+    p = {w->data_ptr(), s->data_ptr()};
+    return true;
+}
+
+// moe_fp8(x, bank, inds, scores, shared or None)
+PyObject* call_moe_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 5) Py_RETURN_NONE;
+    const at::Tensor *x = tensor(args[0]), *inds = tensor(args[2]), *scores = tensor(args[3]), *shared = nullptr;
+    if (!x || !inds || !scores || x->dim() != 3 || inds->dim() != 3 || x->size(0) != inds->size(0) || x->size(1) != inds->size(1) ||
+        !inds->sizes().equals(scores->sizes()) || inds->device() != x->device() || scores->device() != x->device())
+        Py_RETURN_NONE;
+    const int64_t topk = inds->size(2), hidden = x->size(2), rows = x->size(0) * x->size(1);
+    const int dt = act_dtype(*x), sdt = act_dtype(*scores);
+    if (topk <= 0 || topk > T3_REDUCE_MAX_TOPK || rows < 1 || dt < 0 || sdt < 0 || !is_index(*inds)) Py_RETURN_NONE;
+    t3_fp8_bank bank = {};
+    int64_t g[3], u[3], d[3];
+    if (!fp8_proj_of(args[1], s_gate, x->device(), bank.gate, g) || !fp8_proj_of(args[1], s_up, x->device(), bank.up, u) ||
+        !fp8_proj_of(args[1], s_down, x->device(), bank.down, d)) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (g[0] < 1 || g[0] > T3_FP8_EXPERTS_MAX || g[2] != hidden || u[0] != g[0] || u[1] != g[1] || u[2] != hidden || d[0] != g[0] ||
+        d[1] != hidden || d[2] != g[1] || hidden > INT32_MAX || g[1] > INT32_MAX)
+        Py_RETURN_NONE;
+    bank.experts = (int)g[0], bank.hidden = (int)hidden, bank.inter = (int)g[1];
+    if (args[4] != Py_None) {
+        shared = tensor(args[4]);
+        if (!shared || shared->scalar_type() != x->scalar_type() || shared->numel() != x->numel() || shared->device() != x->device()) Py_RETURN_NONE;
+    }
+    const c10::cuda::CUDAGuard guard(x->device());
+    const size_t bytes = t3_moe_fp8_workspace_bytes((size_t)rows, (int)topk, &bank);
+    at::Tensor ws = empty({(int64_t)(bytes ? bytes : 1)}, at::kByte, *x), y = empty(x->sizes(), x->scalar_type(), *x);
+    void* stream = stream_of(*x);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = t3_moe_fp8(x->data_ptr(), dt, (size_t)rows, &bank, inds->data_ptr(), scores->data_ptr(), sdt, (int)topk,
+                        shared ? shared->data_ptr() : nullptr, y.data_ptr(), ws.data_ptr(), bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(status, y);
+    END_HANDLE_TH_ERRORS
+}
+
 struct Buffer {
     Py_buffer view = {};
     bool held = false;
@@ -205,6 +362,10 @@ PyObject* call_table_matmul(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
 PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_linear)), METH_FASTCALL, nullptr},
     {"moe", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_moe)), METH_FASTCALL, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_route)), METH_FASTCALL, nullptr},
+    {"quantize_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_quantize_fp8)), METH_FASTCALL, nullptr},
+    {"linear_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_linear_fp8)), METH_FASTCALL, nullptr},
+    {"moe_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_moe_fp8)), METH_FASTCALL, nullptr},
     {"table_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call_table_matmul)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -216,5 +377,6 @@ PyMODINIT_FUNC PyInit__call(void) {
     s_trellis = PyUnicode_InternFromString("trellis"), s_suh = PyUnicode_InternFromString("suh"), s_svh = PyUnicode_InternFromString("svh");
     s_gate = PyUnicode_InternFromString("gate"), s_up = PyUnicode_InternFromString("up"), s_down = PyUnicode_InternFromString("down");
     s_codebook = PyUnicode_InternFromString("codebook"), s_window_bits = PyUnicode_InternFromString("window_bits");
+    s_w = PyUnicode_InternFromString("w"), s_scale = PyUnicode_InternFromString("scale");
     return PyModule_Create(&module);
 }

@@ -1,0 +1,252 @@
+// The C entry points of the 8-bit layers and the router (include/t3.h): admission and launch planning. Every refusal comes before
+// any launch.
+#include <cmath>
+#include <initializer_list>
+
+#include "../../include/t3.h"
+#include "t3_fp8.h"
+#include "t3_internal.h"
+
+namespace t3 {
+namespace {
+
+bool act_ok(int dt) { return dt == T3_F32 || dt == T3_F16 || dt == T3_BF16; }
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
+size_t up256(size_t v) { return (v + 255u) & ~(size_t)255u; }
+int status_of(cudaError_t rc) { return rc == cudaSuccess ? T3_OK : T3_CUDA_ERROR; }
+uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
+
+// Shared memory a CTA may take: where two fit a multiprocessor (228 KB, 1 KB a CTA reserved), and one
+constexpr uint32_t kTwo = 113u * 1024u, kOne = 227u * 1024u;
+constexpr uint32_t kStagesMost = 12;
+
+struct RowsPlan {
+    uint32_t cap, split, slice_max, stages, smem, per_sm;
+    bool quantise;
+};
+
+// Weight tiles in flight: what fits beside the rest, two CTAs a multiprocessor where four tiles a CTA do
+bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots) {
+    for (uint32_t per = p.cap <= 64u ? 2u : 1u; per >= 1u; --per) {
+        const uint32_t room = per == 2u ? kTwo : kOne;
+        uint32_t stages = kStagesMost < units ? kStagesMost : units;
+        stages = stages < 2u ? 2u : stages;
+        while (stages > 1u && fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) --stages;
+        if (fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) continue;
+        if (per == 2u && stages < 4u && stages < units) continue;
+        p.stages = stages, p.per_sm = per;
+        p.smem = fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots);
+        return true;
+    }
+    return false;
+}
+
+constexpr uint32_t kFusedGroups = 64;  // groups of 128 a CTA quantises itself
+
+// K slices: what leaves the fullest multiprocessor the fewest 128-blocks, counting a CTA's fixed part as three of them
+uint32_t pick_slices(uint32_t tiles, uint32_t kbs) {
+    const uint32_t sms = multiprocessors();
+    uint32_t best = 1, cost = ~0u;
+    for (uint32_t s = 1; s <= kFp8SplitMax && s <= kbs; ++s) {
+        const uint32_t c = div_up(tiles * s, sms) * (div_up(kbs, s) + 3u);
+        if (c < cost) cost = c, best = s;
+    }
+    return best;
+}
+
+bool plan_linear(size_t rows, uint32_t in, uint32_t out, bool given, RowsPlan& p) {
+    p.cap = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u ? 64u : 128u;
+    const uint32_t kbs = in / 128u;
+    const uint64_t tiles = (uint64_t)div_up(out, 128u) * ((rows + p.cap - 1u) / p.cap);
+    p.split = tiles >= multiprocessors() ? 1u : pick_slices((uint32_t)tiles, kbs);
+    p.slice_max = div_up(kbs, p.split);
+    p.quantise = !given && p.cap <= 32u && (uint32_t)rows * p.slice_max <= kFusedGroups;
+    return fit(kFp8Linear, p, p.slice_max, 0, 0);
+}
+
+struct LinearWs {
+    size_t scale, total;
+};
+LinearWs linear_ws(size_t rows, uint32_t in) {
+    const size_t q = up256(rows * in);
+    return {q, q + up256(rows * (in / 128u) * 4u)};
+}
+
+bool linear_shape_ok(size_t rows, int in_dim, int out_dim) {
+    if (in_dim <= 0 || out_dim <= 0 || in_dim % 128 != 0 || rows < 1 || rows > kPrefillDenseRowsMax) return false;
+    const size_t widest = (size_t)(in_dim > out_dim ? in_dim : out_dim);
+    return rows <= 0x7FFFFFFFu / widest;
+}
+
+struct MoePlan {
+    RowsPlan up, down;
+    uint32_t used_max, clusters;  // of gate|up
+    size_t h_scale, total;
+};
+
+// resident CTAs of two a multiprocessor by cluster size, and of one (clusters lie inside a group of multiprocessors)
+uint32_t resident(uint32_t per_sm, uint32_t split) {
+    static const uint32_t two[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264}, one[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+    return (per_sm == 2u ? two[split] : one[split]) * multiprocessors() / 148u;
+}
+
+bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
+    const uint32_t cap = rows <= 16u ? 16u : 32u, slots = (uint32_t)rows * (uint32_t)topk;
+    const uint32_t hk = (uint32_t)b.hidden / 128u, ik = (uint32_t)b.inter / 128u;
+    p.used_max = (uint32_t)b.experts < slots ? (uint32_t)b.experts : slots;
+    p.up.cap = p.down.cap = cap;
+    p.up.quantise = true, p.down.quantise = false;
+    // gate|up: enough slices that the experts' tiles fill the device, and that a slice of the quantised rows leaves room for weights
+    const uint32_t tasks = p.used_max * ik;
+    uint32_t s = 1;
+    while (s < kFp8SplitMax && s * 2u <= hk && (tasks * s < 2u * multiprocessors() || div_up(hk, s) * cap * 128u > 32u * 1024u)) s *= 2u;
+    p.up.split = s, p.up.slice_max = div_up(hk, s);
+    if (!fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots)) return false;
+    const uint32_t most = resident(p.up.per_sm, s) / s;
+    p.clusters = tasks < most ? tasks : most;
+    // down: one tile a cluster, as many slices as are resident at once
+    s = 1;
+    for (uint32_t t = 2; t <= kFp8SplitMax; ++t)
+        if (hk * t <= resident(2, t)) s = t;
+    p.down.split = s, p.down.slice_max = 0;
+    if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots)) return false;
+    const size_t h = up256((size_t)p.used_max * cap * (size_t)b.inter);
+    p.h_scale = h;
+    p.total = h + up256((size_t)p.used_max * cap * ik * 4u);
+    return true;
+}
+
+bool bank_shape_ok(const t3_fp8_bank& b) {
+    return b.hidden > 0 && b.inter > 0 && b.hidden % 128 == 0 && b.inter % 128 == 0 && b.experts > 0 && b.experts <= T3_FP8_EXPERTS_MAX &&
+           (size_t)b.experts * (size_t)(b.hidden > b.inter ? b.hidden : b.inter) <= 0x7FFFFFFFu;
+}
+
+}  // namespace
+}  // namespace t3
+
+using namespace t3;
+
+extern "C" {
+
+int t3_route(const void* logits, int dtype, size_t rows, int experts, int topk, int scoring, const void* bias, int groups, int group_topk,
+             int renormalise, float scale, void* inds, void* scores, void* stream) {
+    if (!logits || !inds || !scores) return T3_NULL_POINTER;
+    if (!act_ok(dtype)) return T3_BAD_EXL3_DTYPE;
+    if (scoring != T3_SCORE_SOFTMAX && scoring != T3_SCORE_SIGMOID) return T3_ENGINE_NOT_IMPLEMENTED;
+    if (rows < 1 || rows > 0x7FFFFFFFu || experts < 1 || experts > T3_ROUTE_EXPERTS_MAX || topk < 1 || topk > T3_REDUCE_MAX_TOPK ||
+        groups < 1 || groups > 32 || experts % groups != 0 || group_topk < 1 || group_topk > groups ||
+        topk > experts / groups * group_topk || !std::isfinite(scale))
+        return T3_BAD_EXL3_SHAPE;
+    RouteArgs a = {};
+    a.logits = logits, a.dt = dtype, a.scoring = scoring, a.bias = static_cast<const float*>(bias), a.rows = rows;
+    a.experts = (uint32_t)experts, a.topk = (uint32_t)topk, a.groups = (uint32_t)groups, a.group_topk = (uint32_t)group_topk;
+    a.renormalise = renormalise != 0, a.scale = scale, a.inds = static_cast<int32_t*>(inds), a.scores = static_cast<float*>(scores);
+    count_launches(1);
+    return status_of(launch_route(a, launches_overlap(), static_cast<cudaStream_t>(stream)));
+}
+
+int t3_quantize_fp8(const void* x, int x_dtype, size_t rows, int in_dim, void* q, void* scale, void* stream) {
+    if (!x || !q || !scale) return T3_NULL_POINTER;
+    if (!act_ok(x_dtype)) return T3_BAD_EXL3_DTYPE;
+    if (in_dim <= 0 || in_dim % 128 != 0 || rows < 1 || rows > (size_t)1 << 40 || !on16(x) || !on16(q)) return T3_BAD_EXL3_SHAPE;
+    count_launches(1);
+    return status_of(launch_fp8_quantize(x, x_dtype, rows, (uint32_t)in_dim, static_cast<uint8_t*>(q), static_cast<float*>(scale),
+                                         launches_overlap(), static_cast<cudaStream_t>(stream)));
+}
+
+size_t t3_linear_fp8_workspace_bytes(size_t rows, int in_dim, int out_dim, int x_dtype) {
+    RowsPlan p;
+    if (!act_ok(x_dtype) || !linear_shape_ok(rows, in_dim, out_dim) || !plan_linear(rows, (uint32_t)in_dim, (uint32_t)out_dim, false, p) || p.quantise)
+        return 0;
+    return linear_ws(rows, (uint32_t)in_dim).total;
+}
+
+int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, const void* w, const void* w_scale, int in_dim, int out_dim,
+                  void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const bool given = x_dtype == T3_E4M3;
+    if (!x || !w || !w_scale || !y || (given && !x_scale)) return T3_NULL_POINTER;
+    if ((!given && !act_ok(x_dtype)) || !act_ok(y_dtype)) return T3_BAD_EXL3_DTYPE;
+    if (!linear_shape_ok(rows, in_dim, out_dim) || (!given && x_scale) || !on16(x) || !on16(w) || !on16(y)) return T3_BAD_EXL3_SHAPE;
+    RowsPlan p;
+    if ((rows > T3_DECODE_ROWS_MAX && !prefill_served()) || !plan_linear(rows, (uint32_t)in_dim, (uint32_t)out_dim, given, p)) return T3_ENGINE_NOT_IMPLEMENTED;
+    const bool ahead = !given && !p.quantise;
+    const LinearWs ws = linear_ws(rows, (uint32_t)in_dim);
+    if (ahead) {
+        if (!workspace) return T3_NULL_POINTER;
+        if (workspace_bytes < ws.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return T3_WORKSPACE_TOO_SMALL;
+    }
+    Fp8RowsArgs a = {};
+    a.rows = (uint32_t)rows, a.in = (uint32_t)in_dim, a.out = (uint32_t)out_dim;
+    a.w_scale[0] = static_cast<const float*>(w_scale);
+    a.y = y, a.y_dt = y_dtype, a.split = p.split, a.slice_max = p.slice_max, a.stages = p.stages, a.topk = 0;
+    a.err = device_error_word();
+    Fp8Maps maps = {};
+    if (!make_byte_map(&maps.w[0], w, (uint64_t)out_dim, (uint64_t)in_dim, 128u)) return T3_KERNEL_CREATE_FAILED;
+    const void* q = given ? x : workspace;
+    if (p.quantise) {
+        a.x = x, a.x_dt = x_dtype;
+    } else {
+        a.x_scale = given ? static_cast<const float*>(x_scale) : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scale);
+        if (!make_byte_map(&maps.rows, q, rows, (uint64_t)in_dim, p.cap)) return T3_KERNEL_CREATE_FAILED;
+    }
+    const bool overlap = launches_overlap();
+    note_geometry(rows > T3_DECODE_ROWS_MAX ? 2 : 1, (uint64_t)in_dim, (uint64_t)out_dim, 0, 8);
+    if (ahead) {
+        count_launches(1);
+        if (cudaError_t rc = launch_fp8_quantize(x, x_dtype, rows, (uint32_t)in_dim, static_cast<uint8_t*>(workspace), const_cast<float*>(a.x_scale),
+                                                 overlap, static_cast<cudaStream_t>(stream)))
+            return status_of(rc);
+    }
+    count_launches(1);
+    return status_of(launch_fp8_rows(kFp8Linear, p.cap, maps, a, div_up((uint32_t)out_dim, 128u), (uint32_t)((rows + p.cap - 1u) / p.cap), p.smem,
+                                     overlap, static_cast<cudaStream_t>(stream)));
+}
+
+size_t t3_moe_fp8_workspace_bytes(size_t rows, int topk, const t3_fp8_bank* bank) {
+    MoePlan p;
+    if (!bank || !bank_shape_ok(*bank) || rows < 1 || rows > T3_DECODE_ROWS_MAX || topk < 1 || topk > T3_REDUCE_MAX_TOPK || !plan_moe(rows, topk, *bank, p))
+        return 0;
+    return p.total;
+}
+
+int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank, const void* inds, const void* scores, int scores_dtype,
+               int topk, const void* shared, void* y, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x || !bank || !inds || !scores || !y || !workspace) return T3_NULL_POINTER;
+    for (const t3_fp8_proj* p : {&bank->gate, &bank->up, &bank->down})
+        if (!p->w || !p->scale) return T3_NULL_POINTER;
+    if (!act_ok(x_dtype) || !act_ok(scores_dtype)) return T3_BAD_EXL3_DTYPE;
+    if (!bank_shape_ok(*bank) || rows < 1 || topk < 1 || topk > T3_REDUCE_MAX_TOPK || !on16(x) || !on16(bank->gate.w) || !on16(bank->up.w) ||
+        !on16(bank->down.w))
+        return T3_BAD_EXL3_SHAPE;
+    MoePlan p;
+    if (rows > T3_DECODE_ROWS_MAX || !plan_moe(rows, topk, *bank, p)) return T3_ENGINE_NOT_IMPLEMENTED;
+    if (workspace_bytes < p.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return T3_WORKSPACE_TOO_SMALL;
+    const uint32_t cap = p.up.cap, hidden = (uint32_t)bank->hidden, inter = (uint32_t)bank->inter, experts = (uint32_t)bank->experts;
+    Fp8Maps up = {}, down = {};
+    if (!make_byte_map(&up.w[0], bank->gate.w, (uint64_t)experts * inter, hidden, 128u) ||
+        !make_byte_map(&up.w[1], bank->up.w, (uint64_t)experts * inter, hidden, 128u) ||
+        !make_byte_map(&down.w[0], bank->down.w, (uint64_t)experts * hidden, inter, 128u) ||
+        !make_byte_map(&down.rows, workspace, (uint64_t)p.used_max * cap, inter, cap))
+        return T3_KERNEL_CREATE_FAILED;
+    Fp8RowsArgs a = {};
+    a.x = x, a.x_dt = x_dtype, a.rows = (uint32_t)rows, a.in = hidden, a.out = inter;
+    a.w_scale[0] = static_cast<const float*>(bank->gate.scale), a.w_scale[1] = static_cast<const float*>(bank->up.scale);
+    a.split = p.up.split, a.slice_max = p.up.slice_max, a.stages = p.up.stages;
+    a.inds = static_cast<const uint32_t*>(inds), a.scores = scores, a.score_dt = scores_dtype, a.topk = (uint32_t)topk, a.experts = experts;
+    a.h = static_cast<uint8_t*>(workspace), a.h_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.h_scale);
+    a.err = device_error_word();
+    const bool overlap = launches_overlap();
+    note_geometry(0, hidden, inter, experts, 8);
+    count_launches(1);
+    if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, 1, p.up.smem, overlap, static_cast<cudaStream_t>(stream)))
+        return status_of(rc);
+    Fp8RowsArgs d = a;
+    d.x = nullptr, d.x_scale = a.h_scale, d.in = inter, d.out = hidden;
+    d.w_scale[0] = static_cast<const float*>(bank->down.scale), d.w_scale[1] = nullptr;
+    d.split = p.down.split, d.slice_max = p.down.slice_max, d.stages = p.down.stages;
+    d.shared = shared, d.y = y, d.y_dt = x_dtype;
+    count_launches(1);
+    return status_of(launch_fp8_rows(kFp8Down, cap, down, d, hidden / 128u, 1, p.down.smem, overlap, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

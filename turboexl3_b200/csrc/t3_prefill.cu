@@ -494,6 +494,18 @@ size_t up256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 
 }  // namespace
 
+bool make_byte_map(void* map, const void* base, uint64_t rows, uint64_t bytes, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {bytes, rows};
+    const cuuint64_t strides[1] = {bytes};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t launch_decode_gemm_cb0(const GemmMaps&, const DecodeGemmArgs&, uint32_t units, uint32_t sms, cudaStream_t);
 cudaError_t launch_decode_gemm_cb1(const GemmMaps&, const DecodeGemmArgs&, uint32_t units, uint32_t sms, cudaStream_t);
 cudaError_t launch_decode_gemm(const GemmMaps& maps, const DecodeGemmArgs& a, uint32_t max_units, int codebook, cudaStream_t stream) {
