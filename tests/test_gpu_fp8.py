@@ -216,6 +216,20 @@ def test_moe_a_nan_row_leaves_the_others():
     assert torch.isnan(y[11].float()).all() and torch.equal(y[keep], clean[keep])
 
 
+def test_moe_a_nan_expert_is_its_rows_alone():
+    x = activations(9, 256, torch.bfloat16, 8)
+    b, parts = bank(6, 256, 256, 5)
+    inds = torch.tensor([[i % 5, 5 if i in (2, 7) else (i + 1) % 5] for i in range(9)], dtype=torch.int32, device="cuda")
+    scores = torch.rand(9, 2, device="cuda")
+    clean = check_moe(x, b, parts, inds, scores)
+    b.down.w.view(torch.uint8)[5, 7, :] = 0x7F
+    b.up.scale[5, 1, 0] = math.nan
+    b.down.scale[5, 0, 0] = math.inf
+    y = t3.moe_fp8(x[None], b, inds[None], scores[None])[0]
+    keep = torch.tensor([i not in (2, 7) for i in range(9)])
+    assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[~keep].float()).all()
+
+
 def test_moe_batch_shape_and_refusals():
     b, _ = bank(4, 256, 128, 3)
     x = activations(6, 256, torch.bfloat16, 1).view(2, 3, 256)

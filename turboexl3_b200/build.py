@@ -31,6 +31,7 @@ UNITS = [
     ("t3_api.cu", "t3_api", []),
     ("t3_fp8_api.cu", "t3_fp8_api", []),
     ("t3_fp8_rows.cu", "t3_fp8_rows", []),
+    ("t3_fp8_gemm.cu", "t3_fp8_gemm", []),
     ("t3_fp8_quant.cu", "t3_fp8_quant", []),
     ("t3_route.cu", "t3_route", []),
     ("t3_dequant.cu", "t3_dequant", []),

@@ -55,9 +55,25 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         : "memory");
 }
 
+// (c.x, c.y) += (a0 b0, a1 b1): two f32 multiply-adds in one instruction
+__device__ __forceinline__ void fma2(float2& c, uint32_t a0, uint32_t a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%0, %1};\n\t"
+        "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+        : "+f"(c.x), "+f"(c.y)
+        : "r"(a0), "r"(a1), "f"(b0), "f"(b1));
+}
+
+// load_act past L1
+__device__ __forceinline__ float load_act_cg(const void* p, int dt, size_t i) {
+    if (dt == kF32) return __ldcg(static_cast<const float*>(p) + i);
+    const uint16_t b = __ldcg(static_cast<const unsigned short*>(p) + i);
+    return dt == kF16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+}
+
 // Waits for a barrier phase; gives up after a while, or at once when any wait of the CTA has given up (`dead`): every role then
 // still walks to its end, on values nobody will use, and the error word says so. CLUSTER: what other CTAs of the cluster wrote
-// before their arrivals is visible after it.
+// before their arrivals is visible after it. The loop is a call: these kernels' code comes from memory again for every launch, behind the
+// weights that have passed through L2, and what it does not hold it does not wait for.
 constexpr uint32_t kFp8Tries = 1u << 22;
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
@@ -74,8 +90,8 @@ __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
         done = mbar_try(bar, parity);
     return done != 0u;
 }
-template <bool CLUSTER = false>
-__device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+template <bool CLUSTER>
+__device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kFp8Tries; ++i) {
         if (fp8_try<CLUSTER>(bar, parity)) return;
@@ -83,6 +99,23 @@ __device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile
     }
     *dead = 1u;
     if (err) atomicOr(err, bit);
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+    if (!fp8_try<CLUSTER>(bar, parity)) fp8_wait_slow<CLUSTER>(bar, parity, dead, err, bit);
+}
+
+// `bytes` (4 or 16) from global to shared memory, in this thread's copy group
+template <uint32_t BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if (BYTES == 16u) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits until all but this thread's last N copy groups are in place
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // ---- thread-block clusters ----
@@ -97,13 +130,22 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void peer_store(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// v to another CTA's shared memory; its four bytes count on the barrier there (both addresses of peer_addr). No fence: a release at cluster
+// scope waits for every earlier store of the thread, those to global memory too (4 us a task under a full load of copies). Only in a
+// launch with a cluster: without one the instruction is illegal.
+__device__ __forceinline__ void peer_store(uint32_t addr, float v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void peer_store4(uint32_t addr, float4 v, uint32_t bar) {  // 16 bytes, on a 16-byte boundary
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(__float_as_uint(v.x)),
+                 "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void peer_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // a box on its way into L2 only: harmless ahead of a wait for the stream's previous kernel, whatever that one writes

@@ -1,5 +1,5 @@
 // The 8-bit operators (e4m3 values, one scale for each block of 128): arguments and launches shared by their kernels
-// (t3_fp8_rows.cu, t3_fp8_quant.cu, t3_route.cu) and the entry points (t3_fp8_api.cu).
+// (t3_fp8_rows.cu, t3_fp8_gemm.cu, t3_fp8_quant.cu, t3_route.cu) and the entry points (t3_fp8_api.cu).
 #pragma once
 
 #include <cuda.h>
@@ -27,6 +27,7 @@ struct Fp8RowsArgs {
     uint32_t split;        // K slices, CTAs of a cluster
     uint32_t slice_max;    // 128-blocks of the largest slice (linear, gate|up)
     uint32_t stages;       // 128 x 128 weight tiles in flight a CTA
+    uint32_t early;        // linear without x: the rows are the output of this call's launch before this one, which has waited for the weights
     // routed
     const uint32_t* inds;  // [rows, topk]
     const void* scores;
@@ -43,11 +44,27 @@ struct Fp8Maps {
     CUtensorMap rows;  // the e4m3 rows (without x): boxes of 128 values x the tile's columns
 };
 
-// `cap`: columns of a tile (rows of the call it serves): 16, 32, 64 or 128; routed 16 or 32
+// `cap`: columns of a tile (rows of the call it serves): 16 or 32
 uint32_t fp8_rows_smem(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages, uint32_t experts,
                        uint32_t slots);
-cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t row_tiles,
-                            uint32_t smem, bool overlap, cudaStream_t stream);
+cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap,
+                            cudaStream_t stream);
+
+// The linear past 32 rows (t3_fp8_gemm.cu)
+struct Fp8GemmArgs {
+    const float *x_scale, *w_scale;  // [rows, in / 128], [out / 128 up, in / 128]
+    void* y;                         // [rows, out] in y_dt
+    int y_dt;
+    uint32_t rows, in, out;
+    uint32_t split;                  // K slices, CTAs of a cluster
+    uint32_t early;                  // as Fp8RowsArgs::early
+    uint32_t* err;
+};
+struct Fp8GemmPlan {
+    uint32_t n, split, grid;  // outputs of a tile (its map's box is that many rows of the weight), K slices, CTAs
+};
+Fp8GemmPlan plan_fp8_gemm(uint32_t rows, uint32_t in, uint32_t out);
+cudaError_t launch_fp8_gemm(const CUtensorMap& w, const CUtensorMap& x, const Fp8GemmArgs& a, const Fp8GemmPlan& p, bool overlap, cudaStream_t stream);
 
 // x [rows, in] -> e4m3 values and scales [rows, in / 128]
 cudaError_t launch_fp8_quantize(const void* x, int dt, size_t rows, uint32_t in, uint8_t* q, float* scale, bool overlap, cudaStream_t stream);

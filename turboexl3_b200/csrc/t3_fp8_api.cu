@@ -27,11 +27,11 @@ struct RowsPlan {
 
 // Weight tiles in flight: what fits beside the rest, two CTAs a multiprocessor where four tiles a CTA do
 bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots) {
-    for (uint32_t per = p.cap <= 64u ? 2u : 1u; per >= 1u; --per) {
+    for (uint32_t per = 2u; per >= 1u; --per) {
         const uint32_t room = per == 2u ? kTwo : kOne;
         uint32_t stages = kStagesMost < units ? kStagesMost : units;
         stages = stages < 2u ? 2u : stages;
-        while (stages > 1u && fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) --stages;
+        while (stages > 2u && fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) --stages;
         if (fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) continue;
         if (per == 2u && stages < 4u && stages < units) continue;
         p.stages = stages, p.per_sm = per;
@@ -54,13 +54,13 @@ uint32_t pick_slices(uint32_t tiles, uint32_t kbs) {
     return best;
 }
 
+// up to T3_DECODE_ROWS_MAX rows
 bool plan_linear(size_t rows, uint32_t in, uint32_t out, bool given, RowsPlan& p) {
-    p.cap = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u ? 64u : 128u;
-    const uint32_t kbs = in / 128u;
-    const uint64_t tiles = (uint64_t)div_up(out, 128u) * ((rows + p.cap - 1u) / p.cap);
-    p.split = tiles >= multiprocessors() ? 1u : pick_slices((uint32_t)tiles, kbs);
+    p.cap = rows <= 16u ? 16u : 32u;
+    const uint32_t kbs = in / 128u, tiles = div_up(out, 128u);
+    p.split = tiles >= multiprocessors() ? 1u : pick_slices(tiles, kbs);
     p.slice_max = div_up(kbs, p.split);
-    p.quantise = !given && p.cap <= 32u && (uint32_t)rows * p.slice_max <= kFusedGroups;
+    p.quantise = !given && (uint32_t)rows * p.slice_max <= kFusedGroups;
     return fit(kFp8Linear, p, p.slice_max, 0, 0);
 }
 
@@ -96,10 +96,10 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     p.used_max = (uint32_t)b.experts < slots ? (uint32_t)b.experts : slots;
     p.up.cap = p.down.cap = cap;
     p.up.quantise = true, p.down.quantise = false;
-    // gate|up: enough slices that the experts' tiles fill the device, and that a slice of the quantised rows leaves room for weights
+    // gate|up: four slices, or the eight that still are resident at once; as many as leave the quantised rows' slice room for weights
     const uint32_t tasks = p.used_max * ik;
     uint32_t s = 1;
-    while (s < kFp8SplitMax && s * 2u <= hk && (tasks * s < 2u * multiprocessors() || div_up(hk, s) * cap * 128u > 32u * 1024u)) s *= 2u;
+    while (s < kFp8SplitMax && s * 2u <= hk && (s < 4u || tasks * s * 2u <= resident(2, s * 2u) || div_up(hk, s) * cap * 128u > 32u * 1024u)) s *= 2u;
     p.up.split = s, p.up.slice_max = div_up(hk, s);
     if (!fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots)) return false;
     const uint32_t most = resident(p.up.per_sm, s) / s;
@@ -155,51 +155,54 @@ int t3_quantize_fp8(const void* x, int x_dtype, size_t rows, int in_dim, void* q
 }
 
 size_t t3_linear_fp8_workspace_bytes(size_t rows, int in_dim, int out_dim, int x_dtype) {
+    if (!act_ok(x_dtype) || !linear_shape_ok(rows, in_dim, out_dim)) return 0;
     RowsPlan p;
-    if (!act_ok(x_dtype) || !linear_shape_ok(rows, in_dim, out_dim) || !plan_linear(rows, (uint32_t)in_dim, (uint32_t)out_dim, false, p) || p.quantise)
-        return 0;
+    if (rows <= T3_DECODE_ROWS_MAX && plan_linear(rows, (uint32_t)in_dim, (uint32_t)out_dim, false, p) && p.quantise) return 0;
     return linear_ws(rows, (uint32_t)in_dim).total;
 }
 
 int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, const void* w, const void* w_scale, int in_dim, int out_dim,
-                  void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    const bool given = x_dtype == T3_E4M3;
+                  void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream_v) {
+    const bool given = x_dtype == T3_E4M3, few = rows <= T3_DECODE_ROWS_MAX;
     if (!x || !w || !w_scale || !y || (given && !x_scale)) return T3_NULL_POINTER;
     if ((!given && !act_ok(x_dtype)) || !act_ok(y_dtype)) return T3_BAD_EXL3_DTYPE;
     if (!linear_shape_ok(rows, in_dim, out_dim) || (!given && x_scale) || !on16(x) || !on16(w) || !on16(y)) return T3_BAD_EXL3_SHAPE;
-    RowsPlan p;
-    if ((rows > T3_DECODE_ROWS_MAX && !prefill_served()) || !plan_linear(rows, (uint32_t)in_dim, (uint32_t)out_dim, given, p)) return T3_ENGINE_NOT_IMPLEMENTED;
-    const bool ahead = !given && !p.quantise;
-    const LinearWs ws = linear_ws(rows, (uint32_t)in_dim);
+    if (!few && !prefill_served()) return T3_ENGINE_NOT_IMPLEMENTED;
+    const uint32_t in = (uint32_t)in_dim, out = (uint32_t)out_dim;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    RowsPlan p = {};
+    Fp8GemmPlan g = {};
+    if (!few) g = plan_fp8_gemm((uint32_t)rows, in, out);
+    else if (!plan_linear(rows, in, out, given, p)) return T3_ENGINE_NOT_IMPLEMENTED;
+    const bool ahead = !given && !p.quantise;  // a launch quantises the rows ahead of the product
+    const LinearWs ws = linear_ws(rows, in);
     if (ahead) {
         if (!workspace) return T3_NULL_POINTER;
         if (workspace_bytes < ws.total || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return T3_WORKSPACE_TOO_SMALL;
     }
-    Fp8RowsArgs a = {};
-    a.rows = (uint32_t)rows, a.in = (uint32_t)in_dim, a.out = (uint32_t)out_dim;
-    a.w_scale[0] = static_cast<const float*>(w_scale);
-    a.y = y, a.y_dt = y_dtype, a.split = p.split, a.slice_max = p.slice_max, a.stages = p.stages, a.topk = 0;
-    a.err = device_error_word();
+    float* scale = given ? static_cast<float*>(const_cast<void*>(x_scale)) : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scale);
     Fp8Maps maps = {};
-    if (!make_byte_map(&maps.w[0], w, (uint64_t)out_dim, (uint64_t)in_dim, 128u)) return T3_KERNEL_CREATE_FAILED;
-    const void* q = given ? x : workspace;
-    if (p.quantise) {
-        a.x = x, a.x_dt = x_dtype;
-    } else {
-        a.x_scale = given ? static_cast<const float*>(x_scale) : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scale);
-        if (!make_byte_map(&maps.rows, q, rows, (uint64_t)in_dim, p.cap)) return T3_KERNEL_CREATE_FAILED;
-    }
+    if (!make_byte_map(&maps.w[0], w, out, in, few ? 128u : g.n)) return T3_KERNEL_CREATE_FAILED;
+    if (!p.quantise && !make_byte_map(&maps.rows, given ? x : workspace, rows, in, few ? p.cap : 128u)) return T3_KERNEL_CREATE_FAILED;
     const bool overlap = launches_overlap();
-    note_geometry(rows > T3_DECODE_ROWS_MAX ? 2 : 1, (uint64_t)in_dim, (uint64_t)out_dim, 0, 8);
+    note_geometry(few ? 1 : 2, in, out, 0, 8);
     if (ahead) {
         count_launches(1);
-        if (cudaError_t rc = launch_fp8_quantize(x, x_dtype, rows, (uint32_t)in_dim, static_cast<uint8_t*>(workspace), const_cast<float*>(a.x_scale),
-                                                 overlap, static_cast<cudaStream_t>(stream)))
-            return status_of(rc);
+        if (cudaError_t rc = launch_fp8_quantize(x, x_dtype, rows, in, static_cast<uint8_t*>(workspace), scale, overlap, stream)) return status_of(rc);
     }
     count_launches(1);
-    return status_of(launch_fp8_rows(kFp8Linear, p.cap, maps, a, div_up((uint32_t)out_dim, 128u), (uint32_t)((rows + p.cap - 1u) / p.cap), p.smem,
-                                     overlap, static_cast<cudaStream_t>(stream)));
+    if (!few) {
+        Fp8GemmArgs a = {};
+        a.x_scale = scale, a.w_scale = static_cast<const float*>(w_scale), a.y = y, a.y_dt = y_dtype;
+        a.rows = (uint32_t)rows, a.in = in, a.out = out, a.split = g.split, a.early = ahead, a.err = device_error_word();
+        return status_of(launch_fp8_gemm(maps.w[0], maps.rows, a, g, overlap, stream));
+    }
+    Fp8RowsArgs a = {};
+    if (p.quantise) a.x = x, a.x_dt = x_dtype;
+    else a.x_scale = scale;
+    a.rows = (uint32_t)rows, a.in = in, a.out = out, a.w_scale[0] = static_cast<const float*>(w_scale);
+    a.y = y, a.y_dt = y_dtype, a.split = p.split, a.slice_max = p.slice_max, a.stages = p.stages, a.early = ahead, a.err = device_error_word();
+    return status_of(launch_fp8_rows(kFp8Linear, p.cap, maps, a, div_up(out, 128u), p.smem, overlap, stream));
 }
 
 size_t t3_moe_fp8_workspace_bytes(size_t rows, int topk, const t3_fp8_bank* bank) {
@@ -238,7 +241,7 @@ int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank,
     const bool overlap = launches_overlap();
     note_geometry(0, hidden, inter, experts, 8);
     count_launches(1);
-    if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, 1, p.up.smem, overlap, static_cast<cudaStream_t>(stream)))
+    if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, p.up.smem, overlap, static_cast<cudaStream_t>(stream)))
         return status_of(rc);
     Fp8RowsArgs d = a;
     d.x = nullptr, d.x_scale = a.h_scale, d.in = inter, d.out = hidden;
@@ -246,7 +249,7 @@ int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank,
     d.split = p.down.split, d.slice_max = p.down.slice_max, d.stages = p.down.stages;
     d.shared = shared, d.y = y, d.y_dt = x_dtype;
     count_launches(1);
-    return status_of(launch_fp8_rows(kFp8Down, cap, down, d, hidden / 128u, 1, p.down.smem, overlap, static_cast<cudaStream_t>(stream)));
+    return status_of(launch_fp8_rows(kFp8Down, cap, down, d, hidden / 128u, p.down.smem, overlap, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

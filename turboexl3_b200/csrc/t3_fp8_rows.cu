@@ -1,24 +1,29 @@
-// Products with e4m3 weights that stream past few rows: the linear up to 128 rows a tile, and the routed layer's two launches.
+// Products with e4m3 weights that stream past few rows (up to 32): the linear, and the routed layer's two launches.
 //
 //   y[n, o] = sum over 128-blocks k of  c[n, k, o / 128] * sum over the block of q[n, i] w[o, i],     c = x scale * w scale
 //
 // The product is taken transposed: a unit of work is a 128 x 128 block of the weight (the A operand, 128 outputs by 128 inputs,
-// K-major as it lies in memory) against the same 128 inputs of the rows (B, 16 to 128 of them), so D [128 outputs x rows] lies in
+// K-major as it lies in memory) against the same 128 inputs of the rows (B, 16 or 32 of them), so D [128 outputs x rows] lies in
 // tensor memory with an output a lane, and the block's scale and a row's multiply its columns: the epilogue warps add c * D to f32
 // sums in registers, since a scale changes every 128 inputs. Bound by the weight's bytes: a block is 16 KB, 700 cycles of a
-// multiprocessor's share of memory, against 128 cycles of tensor core at 16 rows and some 60 instructions of epilogue.
+// multiprocessor's share of memory, against 128 cycles of tensor core and some 60 instructions of epilogue.
 //
 // K is cut into slices, a CTA of a thread-block cluster each; the slices' sums meet in the cluster's shared memory, each CTA
 // adding the columns n = rank, rank + split, .. in slice order, so the result does not depend on timing.
 //
-// Eight warps: 0-3 epilogue (32 outputs each), 4 TMA, 5 tcgen05.mma, 6 the columns' scales, 7 helps quantising. With QUANT the
-// CTAs quantise the rows themselves (their own slice of them) while the first weights are on their way.
+// Twelve warps: 0-3 and 4-7 epilogue, 32 outputs a warp, the fours taking turns at the blocks (one four was what bounded the kernel: 840 cycles a
+// block of 32 columns, most of it the latency of a chain of small steps), 8 TMA, 9 tcgen05.mma, 10 and 11 the columns' scales of each
+// four's blocks. With QUANT the CTAs quantise the rows themselves (their own slice of them), ahead of their weights' copies into
+// shared memory: loads of rows behind a full queue of those took 21 us instead of 2.
+//
+// The code is kept short: what is executed once a launch or once a task comes from memory, since the weights have pushed it out of L2 and
+// the loops out of the nearer caches. An exchange unrolled over the columns took 6000 cycles a task for one or two stores.
 //
 // The routed layer (rows <= 32): gate|up's unit of work for an expert is the same block against ALL rows of the call, whichever of them the
-// router sent there: columns cost nothing here, and no row is gathered. gate|up's tile is 128 channels of gate and of up; its CTAs
-// quantise silu(gate) * up and leave it as e4m3 for the rows that chose the expert. Down's tile is 128 outputs over all experts in
-// use (K runs over expert and input), the router's weight in c, so the sum over a row's experts is taken in registers in
-// ascending order of the experts' numbers: no atomics, no third launch.
+// router sent there: columns cost nothing here, and no row is gathered. gate|up's tile is 128 channels of gate (the first four's) and
+// of up (the second's); its CTAs quantise silu(gate) * up and leave it as e4m3 for the rows that chose the expert. Down's tile is 128
+// outputs over all experts in use (K runs over expert and input), the router's weight in c, so the sum over a row's experts is
+// taken in registers in ascending order of the experts' numbers: no atomics, no third launch.
 #include <type_traits>
 
 #include "t3_fp8.cuh"
@@ -28,16 +33,20 @@
 namespace t3 {
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kTmaWarp = 4, kMmaWarp = 5, kScaleWarp = 6;
+constexpr uint32_t kWarps = 12, kThreads = 32u * kWarps;
+constexpr uint32_t kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;  // and 11
 constexpr uint32_t kTileBytes = 128u * 128u;
 constexpr uint32_t kStagesMax = 12;
+constexpr uint32_t kAcc = 4;      // accumulators in tensor memory; even: one is always the same four's
+constexpr uint32_t kAhead = 8;    // units a scale warp's fetches run ahead of their use (a trip to memory is four or five units long)
+constexpr uint32_t kFull = 0xFFFFFFFFu;
 
-constexpr uint32_t acc_slots(uint32_t cap) { return cap <= 32u ? 4u : 2u; }
+// down: the most experts one of `split` slices of `used` experts' inputs touches
+__host__ __device__ constexpr uint32_t slice_experts(uint32_t used, uint32_t split) { return (used + split - 1u) / split + 1u; }
 
 // Shared memory of a CTA, offsets from a 1024-byte boundary
 struct Layout {
-    uint32_t ring, rows, part, red, sx, c, mask, list, slots, bars, total;
+    uint32_t ring, rows, part, hid, red, sx, fetch, c, mask, list, chunks, slots, weight, bars, total;
 };
 __host__ __device__ __forceinline__ Layout layout_of(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages,
                                                      uint32_t experts, uint32_t slots) {
@@ -48,90 +57,148 @@ __host__ __device__ __forceinline__ Layout layout_of(int mode, uint32_t cap, boo
         at += (bytes + 15u) & ~15u;
         return o;
     };
-    const uint32_t own = (cap + split - 1u) / split;  // columns a CTA adds up
+    const uint32_t own = (cap + split - 1u) / split, used = experts < slots ? experts : slots;  // own: columns a CTA adds up
+    const bool gate_up = mode == kFp8GateUp, routed = mode != kFp8Linear, down = mode == kFp8Down;
     l.ring = take(stages * (kTileBytes + (quantise ? 0u : cap * 128u)));
     l.rows = take(quantise ? slice_max * cap * 128u : 0u);
-    l.part = take(mode == kFp8GateUp ? split * own * 2u * 512u : split > 1u ? split * own * 512u : 0u);
-    l.red = take(mode == kFp8GateUp ? own * 16u : 0u);
+    l.part = take(split * own * (gate_up ? 1024u : 512u));
+    l.hid = take(gate_up ? own * 512u : 0u);
+    l.red = take(gate_up ? own * 16u : 0u);
     l.sx = take(quantise ? slice_max * cap * 4u : 0u);
-    l.c = take(acc_slots(cap) * cap * 4u);
-    l.mask = take(mode == kFp8Linear ? 0u : experts * 4u);
-    l.list = take(mode == kFp8Linear ? 0u : (experts < slots ? experts : slots) * 8u);
-    l.slots = take(mode == kFp8Down ? slots * 8u : 0u);
+    l.fetch = take(2u * kAhead * 33u * 4u);
+    l.c = take(kAcc * cap * 4u);
+    l.mask = take(routed ? experts * 4u : 0u);
+    l.list = take(routed ? used * 8u : 0u);
+    l.chunks = take(routed ? 256u : 0u);  // a word for each 32 experts
+    l.slots = take(down ? slots * 8u : 0u);
+    l.weight = take(down ? slice_experts(used, split) * cap * 4u : 0u);
     l.bars = take(512u);
     l.total = at;
     return l;
 }
 
 // places in Layout::bars
-constexpr uint32_t kBarFull = 0, kBarEmpty = 8u * kStagesMax, kBarAccFull = 16u * kStagesMax, kBarAccEmpty = kBarAccFull + 32u,
-                   kBarRecvFull = kBarAccEmpty + 32u, kBarRecvEmpty = kBarRecvFull + 8u, kWords = kBarRecvEmpty + 8u;
+constexpr uint32_t kBarFull = 0, kBarEmpty = 8u * kStagesMax, kBarAccFull = 16u * kStagesMax, kBarAccEmpty = kBarAccFull + 8u * kAcc,
+                   kBarRecvFull = kBarAccEmpty + 8u * kAcc, kBarRecvEmpty = kBarRecvFull + 8u, kWords = kBarRecvEmpty + 8u;
 static_assert(kWords + 16u <= 512u, "barriers and words");
 
+// a place in a ring and the parity of its round
 struct Slot {
-    uint32_t i = 0, parity = 0;
-    __device__ __forceinline__ void next(uint32_t n) {
-        if (++i == n) i = 0, parity ^= 1u;
+    uint32_t i, parity = 0;
+    __device__ __forceinline__ explicit Slot(uint32_t first = 0) : i(first) {}
+    __device__ __forceinline__ void next(uint32_t n, uint32_t by = 1) {
+        i += by;
+        if (i >= n) i -= n, parity ^= 1u;
     }
 };
 
 // The experts in use, ascending, each with the rows that chose it (a bit a row); ids outside the bank are nobody's. Returns how many.
-__device__ __forceinline__ uint32_t list_experts(const Fp8RowsArgs& a, uint32_t* mask, uint2* list, uint32_t* count) {
+// The routing is read past L1: with the kernel before this one still running, by its own wait complete, but not known to this CTA's cache.
+__device__ __forceinline__ uint32_t list_experts(const Fp8RowsArgs& a, uint32_t* mask, uint2* list, uint32_t* chunks, uint32_t* count) {
+    const uint32_t slots = a.rows * a.topk, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    if (slots <= 32u) {  // one warp, a slot a lane, against every other slot (a token's call: 1.5 us by the general way below)
+        if (warp == 0) {
+            uint32_t e = lane < slots ? __ldcg(a.inds + lane) : kFull;
+            if (e >= a.experts) e = kFull;
+            uint32_t rows = 0, smaller = 0;
+            bool first = e != kFull;
+#pragma unroll 1
+            for (uint32_t t = 0, row = 0, k = 0; t < slots; ++t) {
+                const uint32_t other = __shfl_sync(kFull, e, t);
+                if (other == e) {
+                    rows |= 1u << row;
+                    if (t < lane) first = false;
+                }
+                if (++k == a.topk) k = 0, ++row;
+            }
+            const uint32_t firsts = __ballot_sync(kFull, first);
+#pragma unroll 1
+            for (uint32_t t = 0; t < slots; ++t) {
+                const uint32_t other = __shfl_sync(kFull, e, t);
+                smaller += ((firsts >> t) & 1u) && other < e;
+            }
+            if (first) list[smaller] = make_uint2(e, rows);
+            if (lane == 0) *count = __popc(firsts);
+        }
+        __syncthreads();
+        return *count;
+    }
+#pragma unroll 1
     for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) mask[e] = 0u;
     __syncthreads();
-    for (uint32_t s = threadIdx.x; s < a.rows * a.topk; s += kThreads) {
-        const uint32_t e = a.inds[s];
+#pragma unroll 1
+    for (uint32_t s = threadIdx.x; s < slots; s += kThreads) {
+        const uint32_t e = __ldcg(a.inds + s);
         if (e < a.experts) atomicOr(&mask[e], 1u << (s / a.topk));
     }
     __syncthreads();
-    if (threadIdx.x < 32u) {
-        uint32_t at = 0;
-        for (uint32_t e0 = 0; e0 < a.experts; e0 += 32u) {
-            const uint32_t e = e0 + threadIdx.x, m = e < a.experts ? mask[e] : 0u;
-            const uint32_t used = __ballot_sync(0xFFFFFFFFu, m != 0u);
-            if (m != 0u) list[at + __popc(used & ((1u << threadIdx.x) - 1u))] = make_uint2(e, m);
-            at += __popc(used);
-        }
-        if (threadIdx.x == 0) *count = at;
+    const uint32_t runs = (a.experts + 31u) / 32u;  // at most 64
+    static_assert(kFp8ExpertsMax <= 64u * 32u, "two words a lane");
+#pragma unroll 1
+    for (uint32_t r = warp; r < runs; r += kWarps) {
+        const uint32_t e = r * 32u + lane, in_use = __ballot_sync(kFull, e < a.experts && mask[e] != 0u);
+        if (lane == 0) chunks[r] = __popc(in_use);
+    }
+    __syncthreads();
+    const uint32_t n0 = lane < runs ? chunks[lane] : 0u, n1 = lane + 32u < runs ? chunks[lane + 32u] : 0u;
+#pragma unroll 1
+    for (uint32_t r = warp; r < runs; r += kWarps) {
+        const uint32_t at = __reduce_add_sync(kFull, (lane < r ? n0 : 0u) + (lane + 32u < r ? n1 : 0u));
+        const uint32_t e = r * 32u + lane, m = e < a.experts ? mask[e] : 0u, in_use = __ballot_sync(kFull, m != 0u);
+        if (m != 0u) list[at + __popc(in_use & ((1u << lane) - 1u))] = make_uint2(e, m);
+    }
+    if (warp == 0) {
+        const uint32_t all = __reduce_add_sync(kFull, n0 + n1);
+        if (lane == 0) *count = all;
     }
     __syncthreads();
     return *count;
 }
 
+// sum n of a warp's (n the same in all lanes): a select tree, so that the loop around it is short
+template <uint32_t CAP>
+__device__ __forceinline__ float pick(const float2 (&sums)[CAP / 2u], uint32_t n) {
+    float t[CAP / 2u];
+#pragma unroll
+    for (uint32_t i = 0; i < CAP / 2u; ++i) t[i] = n & 1u ? sums[i].y : sums[i].x;
+#pragma unroll
+    for (uint32_t w = CAP / 4u, bit = CAP / 2u; w >= 1u; w >>= 1, bit >>= 1)
+#pragma unroll
+        for (uint32_t i = 0; i < w; ++i) t[i] = n & bit ? t[i + w] : t[i];
+    return t[0];
+}
+
 template <int MODE, uint32_t CAP, bool QUANT>
-__global__ void __launch_bounds__(kThreads, CAP <= 64u ? 2 : 1) fp8_rows(const __grid_constant__ Fp8Maps maps, const __grid_constant__ Fp8RowsArgs a) {
-    constexpr uint32_t kAcc = acc_slots(CAP), kCols = kAcc * CAP;
-    constexpr uint32_t kIdesc = idesc_m128(CAP);
+__global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ Fp8Maps maps, const __grid_constant__ Fp8RowsArgs a) {
+    constexpr uint32_t kCols = kAcc * CAP, kIdesc = idesc_m128(CAP);
     constexpr uint32_t kStageBytes = kTileBytes + (QUANT ? 0u : CAP * 128u);
-    constexpr uint32_t kSums = MODE == kFp8GateUp ? 2u : 1u;
+    constexpr uint32_t kOps = MODE == kFp8GateUp ? 2u : 1u;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
     const Layout l = layout_of(MODE, CAP, QUANT, a.slice_max, a.split, a.stages, a.experts, a.rows * a.topk);
     const uint32_t base = smem_addr(smem), bars = base + l.bars;
-    volatile uint32_t* dead = reinterpret_cast<uint32_t*>(smem + l.bars + kWords);
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + l.bars + kWords);  // dead, tensor memory, experts in use
+    volatile uint32_t* dead = words;
     float* sx = reinterpret_cast<float*>(smem + l.sx);
-    float* cs = reinterpret_cast<float*>(smem + l.c);
     uint2* list = reinterpret_cast<uint2*>(smem + l.list);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t rank = a.split > 1u ? cluster_rank() : 0u, cluster = blockIdx.x / a.split, clusters = gridDim.x / a.split;
-    const uint32_t kbs = a.in / 128u, tiles = (a.out + 127u) / 128u;
-    const uint32_t row0 = blockIdx.y * CAP, live = min(CAP, a.rows - row0);
+    const uint32_t kbs = a.in / 128u, tiles = (a.out + 127u) / 128u, live = a.rows;
 
-    if (threadIdx.x == 0) {
-        words[0] = 0u;
+    if (warp == 0) {  // a barrier a lane: one thread for all of them took half a microsecond
+        if (lane == 0) words[0] = 0u;
         auto init = [&](uint32_t at, uint32_t n) { mbar_init(reinterpret_cast<uint64_t*>(smem + l.bars + at), n); };
-        for (uint32_t s = 0; s < a.stages; ++s) init(kBarFull + 8u * s, 1), init(kBarEmpty + 8u * s, 1);
-        for (uint32_t s = 0; s < kAcc; ++s) init(kBarAccFull + 8u * s, 2), init(kBarAccEmpty + 8u * s, 4);
-        init(kBarRecvFull, 4u * a.split), init(kBarRecvEmpty, 4u * a.split);
+        if (lane < a.stages) init(kBarFull + 8u * lane, 1), init(kBarEmpty + 8u * lane, 1);
+        if (lane < kAcc) init(kBarAccFull + 8u * lane, 2), init(kBarAccEmpty + 8u * lane, 4);
+        if (lane == 31u) init(kBarRecvFull, 1), init(kBarRecvEmpty, kEpiWarps * a.split);
         mbar_init_fence();
-    }
-    if (warp == kTmaWarp) {
+    } else if (warp == kTmaWarp) {
         if (lane == 0) {
             prefetch_map(&maps.w[0]);
             if (MODE == kFp8GateUp) prefetch_map(&maps.w[1]);
             if (!QUANT) prefetch_map(&maps.rows);
-            if (MODE == kFp8Linear)  // into L2 only, which holds whatever the kernels before this one write
+            if (MODE == kFp8Linear && !a.early)  // into L2 only, which holds whatever the kernels before this one write
+#pragma unroll 1
                 for (uint32_t kb = kbs * rank / a.split, i = 0; kb < kbs * (rank + 1u) / a.split && i < a.stages; ++kb, ++i)
                     tma_prefetch_2d(&maps.w[0], (int)(kb * 128u), (int)(cluster * 128u));
         }
@@ -143,254 +210,337 @@ __global__ void __launch_bounds__(kThreads, CAP <= 64u ? 2 : 1) fp8_rows(const _
     tc_fence_after();
     const uint32_t tmem = words[1];
     if (a.split > 1u) cluster_arrive();  // (waited for ahead of the first store to another CTA)
-    pdl_trigger();                       // after the tensor memory is this CTA's: a later kernel's CTAs may hold theirs while they wait
-    pdl_wait();
-
-    uint32_t used = 1;
-    if (MODE != kFp8Linear) used = list_experts(a, reinterpret_cast<uint32_t*>(smem + l.mask), list, &words[2]);
-    if (MODE == kFp8Down) {  // the routing, for the columns' weights
-        uint2* slots = reinterpret_cast<uint2*>(smem + l.slots);
-        for (uint32_t s = threadIdx.x; s < a.rows * a.topk; s += kThreads) slots[s] = make_uint2(a.inds[s], __float_as_uint(load_act(a.scores, a.score_dt, s)));
-        __syncthreads();
+    // What this kernel reads of the call's earlier launch waits for that one; what was there before the call (`early`: that launch has waited
+    // for it ahead of letting this one start) does not. The next kernel may start once this one's tensor memory is allocated, since its
+    // CTAs may hold theirs while they wait, and this one's own wait is over.
+    const bool early = MODE == kFp8Down || (MODE == kFp8Linear && !QUANT && a.early);
+    if (!early) {
+        pdl_wait();
+        pdl_trigger();
     }
-    if (a.split > 1u) cluster_wait();
 
-    // this CTA's units: of each task (a tile; gate|up: an expert's tile) `units` blocks
-    const uint32_t all = MODE == kFp8Down ? used * kbs : kbs;
-    const uint32_t k0 = (uint32_t)((uint64_t)all * rank / a.split), k1 = (uint32_t)((uint64_t)all * (rank + 1u) / a.split);
-    const uint32_t units = (k1 - k0) * kSums;
-    const uint32_t tasks = MODE == kFp8GateUp ? used * tiles : tiles;
-    struct Unit {
-        uint32_t op, kb, entry;  // the weight (0, or 1 for up), its 128-block of inputs, the expert's place in the list
-    };
-    auto unit_of = [&](uint32_t task, uint32_t i) {
-        Unit u;
-        u.op = MODE == kFp8GateUp ? i & 1u : 0u;
-        const uint32_t k = k0 + (MODE == kFp8GateUp ? i >> 1 : i);
-        u.entry = MODE == kFp8GateUp ? task / tiles : MODE == kFp8Down ? k / kbs : 0u;
-        u.kb = MODE == kFp8Down ? k - u.entry * kbs : k;
-        return u;
-    };
-    auto tile_of = [&](uint32_t task) { return MODE == kFp8GateUp ? task % tiles : task; };
-
-    if (QUANT && warp != kTmaWarp) {
-        // the rows' slice to e4m3, a warp a group, four groups under way: lane's four values to their place in the swizzled tile
-        const uint32_t me = warp < kTmaWarp ? warp : warp - 1u, nb = k1 - k0, groups = live * nb;
-        for (uint32_t g0 = me; g0 < groups; g0 += 7u * 4u) {
-            float v[4][4];
-            uint32_t most[4];
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; ++j) {
-                const uint32_t g = g0 + 7u * j;
-                if (g >= groups) break;
-                const uint32_t n = g / nb, kb = g - n * nb;
-                load_act4(a.x, a.x_dt, (size_t)(row0 + n) * a.in + (k0 + kb) * 128u + 4u * lane, v[j]);
+    if (QUANT) {
+        // The rows' slice to e4m3, a warp a group, a lane's four values to their place in the swizzled tile. The groups come through the ring
+        // (which has no weights yet), a share of it a warp: all of a warp's are on their way at once.
+        const uint32_t q0 = kbs * rank / a.split, nb = kbs * (rank + 1u) / a.split - q0, groups = live * nb;
+        const uint32_t bytes = a.x_dt == kF32 ? 512u : 256u, room = a.stages * kTileBytes / kWarps / bytes, stage = base + l.ring + warp * room * bytes;
+        const uint8_t* x = static_cast<const uint8_t*>(a.x);
+        uint32_t g = warp, n = g / nb, kb = g - n * nb;
+        const uint32_t dn = kWarps / nb, dk = kWarps - dn * nb;
+        auto next = [&](uint32_t& n, uint32_t& kb) {
+            n += dn, kb += dk;
+            if (kb >= nb) kb -= nb, ++n;
+        };
+#pragma unroll 1
+        while (g < groups) {
+            uint32_t m = 0, n2 = n, kb2 = kb;
+#pragma unroll 1
+            for (; m < room && g < groups; ++m, g += kWarps) {
+                if (lane * 16u < bytes) copy_async<16>(stage + m * bytes + lane * 16u, x + ((size_t)n * kbs + q0 + kb) * bytes + lane * 16u);
+                next(n, kb);
             }
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; ++j) {
-                const uint32_t g = g0 + 7u * j;
-                if (g >= groups) break;
-                most[j] = max(max(magnitude(v[j][0]), magnitude(v[j][1])), max(magnitude(v[j][2]), magnitude(v[j][3])));
-                most[j] = __reduce_max_sync(0xFFFFFFFFu, most[j]);
-                const uint32_t n = g / nb, kb = g - n * nb;
-                const float s = fp8_scale(most[j]);
-                const uint32_t q = to_e4m3x4(v[j], s);
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + l.rows + kb * CAP * 128u + n * 128u + (((lane >> 2) ^ (n & 7u)) << 4) +
-                                                             (lane & 3u) * 4u),
-                             "r"(q)
+            copy_commit();
+            copy_wait<0>();
+            __syncwarp();
+#pragma unroll 1
+            for (uint32_t j = 0; j < m; ++j) {
+                float v[4];
+                load_act4(smem + (stage - base) + j * bytes, a.x_dt, 4u * lane, v);
+                uint32_t most = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+                most = __reduce_max_sync(kFull, most);
+                const float s = fp8_scale(most);
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + l.rows + (kb2 * CAP + n2) * 128u + (((lane >> 2) ^ (n2 & 7u)) << 4) + (lane & 3u) * 4u),
+                             "r"(to_e4m3x4(v, s))
                              : "memory");
-                if (lane == 0) sx[kb * CAP + n] = s;
+                if (lane == 0) sx[kb2 * CAP + n2] = s;
+                next(n2, kb2);
             }
+            __syncwarp();
         }
         proxy_fence();
-        named_sync(1, 7u * 32u);
+        if (MODE == kFp8Linear) __syncthreads();  // (list_experts is one)
+    }
+    uint32_t used = 1;
+    if (MODE != kFp8Linear)
+        used = list_experts(a, reinterpret_cast<uint32_t*>(smem + l.mask), list, reinterpret_cast<uint32_t*>(smem + l.chunks), &words[2]);
+
+    // This CTA's units: of each of its tasks (a tile; gate|up: an expert's tile, of which a cluster takes several) `units` blocks. A unit
+    // is (weight, 128-block of inputs, expert's place in the list, tile); they are walked by additions alone, since a division for
+    // each cost the lone warps that walk them more than their waits.
+    const uint32_t all = MODE == kFp8Down ? used * kbs : kbs;
+    const uint32_t k0 = (uint32_t)((uint64_t)all * rank / a.split), k1 = (uint32_t)((uint64_t)all * (rank + 1u) / a.split);
+    const uint32_t units = (k1 - k0) * kOps;
+    const uint32_t tasks = MODE == kFp8GateUp ? used * tiles : tiles;
+    const uint32_t mine = MODE == kFp8GateUp ? (tasks > cluster ? (tasks - cluster + clusters - 1u) / clusters : 0u) : 1u;
+    const uint32_t blocks = mine * units;
+    const uint32_t entry0 = MODE == kFp8Down ? k0 / kbs : MODE == kFp8GateUp ? cluster / tiles : 0u;
+    const uint32_t tile0 = MODE == kFp8GateUp ? cluster - entry0 * tiles : cluster;
+    const uint32_t d_entry = MODE == kFp8GateUp ? clusters / tiles : 0u, d_tile = MODE == kFp8GateUp ? clusters - d_entry * tiles : 0u;
+    struct Walk {
+        uint32_t op, kb, entry, tile;
+    };
+    auto next_task = [&](Walk& u) {
+        u.entry += d_entry, u.tile += d_tile;
+        if (u.tile >= tiles) u.tile -= tiles, ++u.entry;
+    };
+    auto step = [&](Walk& u) {
+        if (MODE == kFp8GateUp && (u.op ^= 1u) != 0u) return;
+        ++u.kb;
+        if (MODE == kFp8Down && u.kb == kbs) u.kb = 0, ++u.entry;
+        if (MODE == kFp8GateUp && u.kb == k1) u.kb = k0, next_task(u);
+    };
+    const Walk begin = {0u, MODE == kFp8Down ? k0 - entry0 * kbs : k0, entry0, tile0};
+
+    float* weight = reinterpret_cast<float*>(smem + l.weight);
+    if (MODE == kFp8Down && units) {
+        // what the router gave each row for each of this slice's experts, over all of the row's slots that name the expert
+        uint2* slots = reinterpret_cast<uint2*>(smem + l.slots);
+#pragma unroll 1
+        for (uint32_t s = threadIdx.x; s < a.rows * a.topk; s += kThreads)
+            slots[s] = make_uint2(__ldcg(a.inds + s), __float_as_uint(load_act_cg(a.scores, a.score_dt, s)));
+        __syncthreads();
+        const uint32_t n = (k1 - 1u) / kbs + 1u - entry0;
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < n * CAP; i += kThreads) {
+            const uint2 e = list[entry0 + i / CAP];
+            const uint32_t r = i % CAP;
+            float v = 0.0f;
+            if ((e.y >> r) & 1u)
+#pragma unroll 1
+                for (uint32_t k = 0; k < a.topk; ++k)
+                    if (slots[r * a.topk + k].x == e.x) v += __uint_as_float(slots[r * a.topk + k].y);
+            weight[i] = v;
+        }
+        __syncthreads();
+    }
+    if (a.split > 1u) {
+        __syncwarp();
+        cluster_wait();
     }
 
     if (warp == kTmaWarp) {
+        // early: first the ring full of weights, then the rows beside them, once the launch that makes them is over
+        const uint32_t ahead = early ? min(a.stages, blocks) : 0u;
         Slot s;
-        for (uint32_t task = cluster; task < tasks; task += clusters) {
-            for (uint32_t i = 0; i < units; ++i) {
-                const Unit u = unit_of(task, i);
-                const uint32_t full = bars + kBarFull + 8u * s.i, at = base + l.ring + s.i * kStageBytes;
-                fp8_wait(bars + kBarEmpty + 8u * s.i, s.parity ^ 1u, dead, a.err, kErrEmptyWait);
-                if (elect_one()) {
-                    const uint32_t bank_row = MODE == kFp8Linear ? 0u : list[u.entry].x * a.out;
-                    mbar_arrive_expect_tx_addr(full, kStageBytes);
-                    tma_load_2d(at, &maps.w[u.op], (int)(u.kb * 128u), (int)(bank_row + tile_of(task) * 128u), full);
-                    if (!QUANT)
-                        tma_load_2d(at + kTileBytes, &maps.rows, (int)(u.kb * 128u), (int)(MODE == kFp8Down ? u.entry * CAP : row0), full);
-                }
-                __syncwarp();
-                s.next(a.stages);
+        Walk u = begin, r = begin;
+#pragma unroll 1
+        for (uint32_t i = 0; i < blocks + ahead; ++i) {
+            const bool rows_only = !QUANT && i >= ahead && i < 2u * ahead;
+            if (!QUANT && early && i == ahead) {
+                pdl_wait();
+                pdl_trigger();
             }
+            const uint32_t slot = rows_only ? i - ahead : s.i;
+            const uint32_t full = bars + kBarFull + 8u * slot, at = base + l.ring + slot * kStageBytes;
+            if (!rows_only) fp8_wait(bars + kBarEmpty + 8u * slot, s.parity ^ 1u, dead, a.err, kErrEmptyWait);
+            if (elect_one()) {
+                if (!rows_only) {
+                    mbar_arrive_expect_tx_addr(full, kStageBytes);
+                    const uint32_t row = (MODE == kFp8Linear ? 0u : list[u.entry].x * a.out) + u.tile * 128u;
+                    tma_load_2d(at, &maps.w[u.op], (int)(u.kb * 128u), (int)row, full);
+                }
+                if (!QUANT && i >= ahead)
+                    tma_load_2d(at + kTileBytes, &maps.rows, (int)(r.kb * 128u), (int)(MODE == kFp8Down ? r.entry * CAP : 0u), full);
+            }
+            __syncwarp();
+            if (!rows_only) {
+                s.next(a.stages);
+                step(u);
+            }
+            if (i >= ahead) step(r);
         }
+        if (early && blocks == 0u) pdl_wait();
     } else if (warp == kMmaWarp) {
         Slot s, c;
-        for (uint32_t task = cluster; task < tasks; task += clusters) {
-            for (uint32_t i = 0; i < units; ++i) {
-                const uint32_t at = base + l.ring + s.i * kStageBytes;
-                const uint32_t rows_at = QUANT ? base + l.rows + (MODE == kFp8GateUp ? i >> 1 : i) * CAP * 128u : at + kTileBytes;
-                const uint64_t ad = umma_desc(at), bd = umma_desc(rows_at);
-                fp8_wait(bars + kBarAccEmpty + 8u * c.i, c.parity ^ 1u, dead, a.err, kErrEmptyWait);
-                fp8_wait(bars + kBarFull + 8u * s.i, s.parity, dead, a.err, kErrFullWait);
+        uint32_t k = 0;  // gate|up, QUANT: the block's place in the slice, each twice
+#pragma unroll 1
+        for (uint32_t i = 0; i < blocks; ++i) {
+            const uint32_t at = base + l.ring + s.i * kStageBytes;
+            const uint64_t ad = umma_desc(at), bd = umma_desc(QUANT ? base + l.rows + k / kOps * CAP * 128u : at + kTileBytes);
+            if (++k == units) k = 0;
+            fp8_wait(bars + kBarAccEmpty + 8u * c.i, c.parity ^ 1u, dead, a.err, kErrEmptyWait);
+            fp8_wait(bars + kBarFull + 8u * s.i, s.parity, dead, a.err, kErrFullWait);
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j)  // 32 inputs each
+                if (elect_one()) umma_e4m3(tmem + c.i * CAP, ad + 2u * j, bd + 2u * j, j, kIdesc);
+            if (elect_one()) {
+                umma_commit(bars + kBarEmpty + 8u * s.i);
+                umma_commit(bars + kBarAccFull + 8u * c.i);
+            }
+            __syncwarp();
+            s.next(a.stages), c.next(kAcc);
+        }
+    } else if (warp >= kScaleWarp) {
+        // The columns' scales of one four's units, a lane a column. What lies in memory (the block's scale; the rows', where they came quantised)
+        // is on its way to shared memory kAhead units before its use.
+        const uint32_t four = warp - kScaleWarp;
+        const uint32_t fetch = l.fetch + four * kAhead * 132u;
+        Walk f = begin, u;
+        if (four) step(f);
+        u = f;
+        if (early) pdl_wait();
+        auto ask = [&](uint32_t i, uint32_t slot) {
+            if (i < blocks) {
+                const uint2 e = MODE == kFp8Linear ? make_uint2(0u, (1u << (live - 1u)) * 2u - 1u) : list[f.entry];
+                const uint32_t to = base + fetch + slot * 132u;
+                if (lane == 0) copy_async<4>(to + 128u, a.w_scale[f.op] + ((size_t)e.x * tiles + f.tile) * kbs + f.kb);
+                if (!QUANT && ((e.y >> lane) & 1u)) copy_async<4>(to + 4u * lane, a.x_scale + ((size_t)(MODE == kFp8Down ? f.entry * CAP : 0u) + lane) * kbs + f.kb);
+                step(f), step(f);
+            }
+            copy_commit();
+        };
+#pragma unroll 1
+        for (uint32_t j = 0; j < kAhead; ++j) ask(four + 2u * j, j);
+        Slot c(four), q;
+#pragma unroll 1
+        for (uint32_t i = four; i < blocks; i += 2u) {
+            copy_wait<(int)kAhead - 1>();
+            __syncwarp();
+            const float* got = reinterpret_cast<const float*>(smem + fetch + q.i * 132u);
+            float v = 0.0f;
+            if (QUANT) {
+                if (lane < CAP) v = sx[(u.kb - k0) * CAP + lane] * got[32];
+            } else {
+                const uint32_t members = MODE == kFp8Down ? list[u.entry].y : (1u << (live - 1u)) * 2u - 1u;
+                if ((members >> lane) & 1u) {  // (the others have no scale)
+                    v = got[lane] * got[32];
+                    if (MODE == kFp8Down) v *= weight[(u.entry - entry0) * CAP + lane];
+                }
+            }
+            __syncwarp();
+            ask(i + 2u * kAhead, q.i);
+            q.next(kAhead);
+            step(u), step(u);
+            fp8_wait(bars + kBarAccEmpty + 8u * c.i, c.parity ^ 1u, dead, a.err, kErrEmptyWait);
+            if (lane < CAP) reinterpret_cast<float*>(smem + l.c)[c.i * CAP + lane] = v;
+            __syncwarp();
+            if (lane == 0) mbar_arrive_addr(bars + kBarAccFull + 8u * c.i);
+            c.next(kAcc, 2);
+        }
+    } else {
+        const uint32_t four = warp >> 2, quarter = warp & 3u, row = quarter * 32u + lane;  // of the tile's 128 outputs
+        const uint32_t own = (CAP + a.split - 1u) / a.split;
+        uint32_t columns = 0;  // a bit for each column this CTA finishes
+#pragma unroll 1
+        for (uint32_t n = rank; n < CAP; n += a.split) columns |= 1u << n;
+        Slot c(four);
+        Walk t = begin;  // gate|up: the task; down: the expert of the unit
+        if (MODE == kFp8Down && four) step(t);
+#pragma unroll 1
+        for (uint32_t turn = 0; turn < mine; ++turn) {
+            float2 sums[CAP / 2u];  // gate|up: of gate (the first four) or of up
+#pragma unroll
+            for (uint32_t n = 0; n < CAP / 2u; ++n) sums[n] = make_float2(0.0f, 0.0f);
+            // Rows that did not choose the expert: their columns are left out by sixteens; in down, where the others' would reach a sum, one by
+            // one too (what lies in the place of such a row, nothing having been written there, or its product with a weight that is a NaN)
+            uint32_t members = MODE == kFp8GateUp ? list[t.entry].y : (1u << (live - 1u)) * 2u - 1u;
+#pragma unroll 1
+            for (uint32_t i = four; i < units; i += 2u) {
+                if (MODE == kFp8Down) members = list[t.entry].y;
+                const uint32_t from = tmem + c.i * CAP + ((quarter * 32u) << 16), cc = base + l.c + c.i * CAP * 4u;
+                fp8_wait(bars + kBarAccFull + 8u * c.i, c.parity, dead, a.err, kErrMmaWait);
                 tc_fence_after();
 #pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k)  // 32 inputs each
-                    if (elect_one()) umma_e4m3(tmem + c.i * CAP, ad + 2u * k, bd + 2u * k, k, kIdesc);
-                if (elect_one()) {
-                    umma_commit(bars + kBarEmpty + 8u * s.i);
-                    umma_commit(bars + kBarAccFull + 8u * c.i);
-                }
-                __syncwarp();
-                s.next(a.stages), c.next(kAcc);
-            }
-        }
-    } else if (warp == kScaleWarp) {
-        // the columns' scales of every unit, fetched a unit ahead of their use
-        constexpr uint32_t kPer = CAP <= 32u ? 1u : CAP / 32u;
-        uint32_t known = 0xFFFFFFFFu;
-        float weight = 0.0f;
-        auto fetch = [&](uint32_t task, uint32_t i, float (&v)[kPer]) {
-            const Unit u = unit_of(task, i);
-            const size_t blk = (size_t)(MODE == kFp8Linear ? 0u : list[u.entry].x) * tiles + tile_of(task);
-            const float sw = __ldg(a.w_scale[u.op] + blk * kbs + u.kb);
+                for (uint32_t b = 0; b < CAP; b += 16u) {
+                    const uint32_t m = members >> b;
+                    if ((m & 0xFFFFu) == 0u) continue;
+                    uint32_t v[16];
+                    float4 f[4];
+                    tmem_ld_32x16(from + b, v);
 #pragma unroll
-            for (uint32_t j = 0; j < kPer; ++j) {
-                const uint32_t n = lane + 32u * j;
-                if (MODE == kFp8Down) {
-                    const uint2 e = list[u.entry];
-                    if (u.entry != known) {  // the row's weight of this expert, over all of its slots that name it
-                        known = u.entry, weight = 0.0f;
-                        const uint2* slots = reinterpret_cast<const uint2*>(smem + l.slots) + lane * a.topk;
-                        if (lane < CAP && ((e.y >> lane) & 1u))
-                            for (uint32_t k = 0; k < a.topk; ++k)
-                                if (slots[k].x == e.x) weight += __uint_as_float(slots[k].y);
-                    }
-                    v[j] = lane < CAP && ((e.y >> lane) & 1u) ? a.x_scale[((size_t)u.entry * CAP + n) * kbs + u.kb] * sw * weight : 0.0f;
-                } else if (QUANT) {
-                    v[j] = n < live ? sx[(u.kb - k0) * CAP + n] * sw : 0.0f;
-                } else {
-                    v[j] = n < live ? __ldg(a.x_scale + (size_t)(row0 + n) * kbs + u.kb) * sw : 0.0f;
-                }
-            }
-        };
-        Slot c;
-        for (uint32_t task = cluster; task < tasks; task += clusters) {
-            float v[kPer];
-            if (units) fetch(task, 0, v);
-            for (uint32_t i = 0; i < units; ++i) {
-                fp8_wait(bars + kBarAccEmpty + 8u * c.i, c.parity ^ 1u, dead, a.err, kErrEmptyWait);
+                    for (uint32_t j = 0; j < 4u; ++j)
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[j].x), "=f"(f[j].y), "=f"(f[j].z), "=f"(f[j].w) : "r"(cc + 4u * b + 16u * j));
+                    tmem_ld_wait(v);
 #pragma unroll
-                for (uint32_t j = 0; j < kPer; ++j)
-                    if (CAP >= 32u || lane < CAP) cs[c.i * CAP + lane + 32u * j] = v[j];
-                __syncwarp();
-                if (lane == 0) mbar_arrive_addr(bars + kBarAccFull + 8u * c.i);
-                c.next(kAcc);
-                if (i + 1u < units) fetch(task, i + 1u, v);
-            }
-        }
-    } else if (warp < kTmaWarp) {
-        const uint32_t row = warp * 32u + lane;  // of the tile's 128 outputs
-        Slot c;
-        uint32_t turn = 0;
-        for (uint32_t task = cluster; task < tasks; task += clusters, ++turn) {
-            float acc[kSums][CAP];
-#pragma unroll
-            for (uint32_t s = 0; s < kSums; ++s)
-#pragma unroll
-                for (uint32_t n = 0; n < CAP; ++n) acc[s][n] = 0.0f;
-            for (uint32_t i = 0; i < units; i += kSums) {
-#pragma unroll
-                for (uint32_t s = 0; s < kSums; ++s) {
-                    fp8_wait(bars + kBarAccFull + 8u * c.i, c.parity, dead, a.err, kErrMmaWait);
-                    tc_fence_after();
-                    const uint32_t from = tmem + c.i * CAP + ((warp * 32u) << 16);
-                    const float* cc = cs + c.i * CAP;
-                    // rows that did not choose the expert have nothing in h: whatever lies there must not reach a sum
-                    const uint32_t members = MODE == kFp8Down ? list[unit_of(task, i).entry].y : 0xFFFFFFFFu;
-#pragma unroll
-                    for (uint32_t b = 0; b < CAP; b += 16u) {
-                        uint32_t v[16];
-                        tmem_ld_32x16(from + b, v);
-                        tmem_ld_wait(v);
-#pragma unroll
-                        for (uint32_t j = 0; j < 16u; j += 4u) {
-                            const float4 f = *reinterpret_cast<const float4*>(cc + b + j);
-                            const float g[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                            for (uint32_t k = 0; k < 4u; ++k)
-                                if (MODE != kFp8Down || ((members >> (b + j + k)) & 1u))
-                                    acc[s][b + j + k] = fmaf(__uint_as_float(v[j + k]), g[k], acc[s][b + j + k]);
+                    for (uint32_t j = 0; j < 4u; ++j) {
+                        float2 &lo = sums[b / 2u + 2u * j], &hi = sums[b / 2u + 2u * j + 1u];
+                        if (MODE == kFp8Down) {
+                            if ((m >> (4u * j)) & 1u) lo.x = fmaf(__uint_as_float(v[4u * j]), f[j].x, lo.x);
+                            if ((m >> (4u * j)) & 2u) lo.y = fmaf(__uint_as_float(v[4u * j + 1u]), f[j].y, lo.y);
+                            if ((m >> (4u * j)) & 4u) hi.x = fmaf(__uint_as_float(v[4u * j + 2u]), f[j].z, hi.x);
+                            if ((m >> (4u * j)) & 8u) hi.y = fmaf(__uint_as_float(v[4u * j + 3u]), f[j].w, hi.y);
+                        } else {
+                            fma2(lo, v[4u * j], v[4u * j + 1u], f[j].x, f[j].y);
+                            fma2(hi, v[4u * j + 2u], v[4u * j + 3u], f[j].z, f[j].w);
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_addr(bars + kBarAccEmpty + 8u * c.i);
-                    c.next(kAcc);
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_addr(bars + kBarAccEmpty + 8u * c.i);
+                c.next(kAcc, 2);
+                if (MODE == kFp8Down) step(t), step(t);
             }
             if (MODE == kFp8GateUp) {
-                // every CTA's sums of column n to the CTA that finishes it (its rank is n mod split), once that has read the last task's
-                const uint2 e = list[task / tiles];
-                const uint32_t own = (CAP + a.split - 1u) / a.split;
-                if (turn) fp8_wait<true>(bars + kBarRecvEmpty, (turn - 1u) & 1u, dead, a.err, kErrEmptyWait);
-                uint32_t to = 0, at = base + l.part + rank * own * 1024u + row * 4u;
-#pragma unroll
-                for (uint32_t n = 0; n < CAP; ++n) {
-                    if ((e.y >> n) & 1u) {
-                        const uint32_t p = peer_addr(at, to);
-                        peer_store(p, acc[0][n]);
-                        peer_store(p + 512u, acc[kSums - 1u][n]);
-                    }
-                    if (++to == a.split) to = 0, at += 1024u;
+                // Every CTA's sums of a row that chose the expert to the CTA that finishes it (row n: rank n mod split), in the order of its
+                // rows, once that has read the last task's.
+                const uint32_t full = bars + kBarRecvFull, mine_of = members & columns, count = __popc(mine_of);
+                if (a.split > 1u) {
+                    if (warp == 0 && lane == 0) mbar_arrive_expect_tx_addr(full, count * a.split * 1024u);
+                    if (turn) fp8_wait<true>(bars + kBarRecvEmpty, (turn - 1u) & 1u, dead, a.err, kErrEmptyWait);
+                } else {
+                    named_sync(4, kEpiWarps * 32u);  // (both fours have read the last task's)
                 }
-                __syncwarp();
-                if (lane < a.split) peer_arrive(peer_addr(bars + kBarRecvFull, lane));
-                fp8_wait<true>(bars + kBarRecvFull, turn & 1u, dead, a.err, kErrFullWait);
-                float* part = reinterpret_cast<float*>(smem + l.part);
+                const uint32_t from = base + l.part + rank * own * 1024u + four * 512u + row * 4u;
+#pragma unroll 1
+                for (uint32_t m = members; m; m &= m - 1u) {
+                    const uint32_t n = __ffs(m) - 1u, to = n % a.split;
+                    uint32_t j = 0;  // its place among the rows of that CTA
+#pragma unroll 1
+                    for (uint32_t o = to; o < n; o += a.split) j += (members >> o) & 1u;
+                    const float v = pick<CAP>(sums, n);
+                    if (a.split > 1u)
+                        peer_store(peer_addr(from + j * 1024u, to), v, peer_addr(full, to));
+                    else
+                        *reinterpret_cast<float*>(smem + (from - base) + j * 1024u) = v;
+                }
+                if (a.split > 1u) fp8_wait<true>(full, turn & 1u, dead, a.err, kErrFullWait);
+                else named_sync(4, kEpiWarps * 32u);
+                const float* part = reinterpret_cast<const float*>(smem + l.part) + row;
+                float* hid = reinterpret_cast<float*>(smem + l.hid) + row;
                 uint32_t* red = reinterpret_cast<uint32_t*>(smem + l.red);
-                for (uint32_t j = 0, n = rank; n < CAP; ++j, n += a.split) {
-                    if (!((e.y >> n) & 1u)) continue;
+#pragma unroll 1
+                for (uint32_t j = four; j < count; j += 2u) {  // each four finishes every other of this CTA's rows
                     float g = 0.0f, u = 0.0f;
-                    for (uint32_t s = 0; s < a.split; ++s) {
-                        const float* p = part + (s * own + j) * 256u + row;
-                        g += p[0], u += p[128];
-                    }
+#pragma unroll 1
+                    for (uint32_t s = 0; s < a.split; ++s) g += part[(s * own + j) * 256u], u += part[(s * own + j) * 256u + 128u];
                     const float h = g / (1.0f + expf(-g)) * u;
-                    part[j * 256u + row] = h;  // (slice 0's place: this thread alone reads it)
-                    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, magnitude(h));
-                    if (lane == 0) red[4u * j + warp] = most;
+                    hid[j * 128u] = h;  // (this thread alone reads it)
+                    const uint32_t most = __reduce_max_sync(kFull, magnitude(h));
+                    if (lane == 0) red[4u * j + quarter] = most;
                 }
-                named_sync(2, 128);
-                const uint32_t tile = task % tiles;
-                for (uint32_t j = 0, n = rank; n < CAP; ++j, n += a.split) {
-                    if (!((e.y >> n) & 1u)) continue;
-                    const uint4 m = *reinterpret_cast<const uint4*>(red + 4u * j);
-                    const float s = fp8_scale(max(max(m.x, m.y), max(m.z, m.w)));
-                    const float v[4] = {part[j * 256u + row], 0.0f, 0.0f, 0.0f};
-                    const size_t r = (size_t)(task / tiles) * CAP + n;
-                    a.h[r * a.out + tile * 128u + row] = (uint8_t)to_e4m3x4(v, s);
-                    if (row == 0) a.h_scale[r * tiles + tile] = s;
+                named_sync(2u + four, 128);
+                if (a.split > 1u && lane < a.split) peer_arrive(peer_addr(bars + kBarRecvEmpty, lane));  // ahead of the stores below: a release waits for them
+                uint32_t m = mine_of;
+#pragma unroll 1
+                for (uint32_t j = 0; j < count; ++j, m &= m - 1u) {
+                    if ((j & 1u) != four) continue;
+                    const uint4 r = *reinterpret_cast<const uint4*>(red + 4u * j);
+                    const float s = fp8_scale(max(max(r.x, r.y), max(r.z, r.w)));
+                    const float v[4] = {hid[j * 128u], 0.0f, 0.0f, 0.0f};
+                    const size_t at = (size_t)t.entry * CAP + (__ffs(m) - 1u);
+                    a.h[at * a.out + t.tile * 128u + row] = (uint8_t)to_e4m3x4(v, s);
+                    if (row == 0) a.h_scale[at * tiles + t.tile] = s;
                 }
-                named_sync(2, 128);  // (red is written again for the next task)
-                if (lane < a.split) peer_arrive(peer_addr(bars + kBarRecvEmpty, lane));
-            } else if (a.split > 1u) {
-                const uint32_t own = (CAP + a.split - 1u) / a.split;
-                uint32_t to = 0, at = base + l.part + rank * own * 512u + row * 4u;
-#pragma unroll
-                for (uint32_t n = 0; n < CAP; ++n) {
-                    if (n < live) peer_store(peer_addr(at, to), acc[0][n]);
-                    if (++to == a.split) to = 0, at += 512u;
-                }
+                named_sync(2u + four, 128);  // (red is written again for the next task)
+                next_task(t);
             } else {
-                const uint32_t o = task * 128u + row;
-                if (o < a.out)
+                // both fours' sums over the ring, once every block has been multiplied, and from there to the CTAs that add the slices up
+                float* mid = reinterpret_cast<float*>(smem + l.ring) + row;
+                named_sync(4, kEpiWarps * 32u);
 #pragma unroll
-                    for (uint32_t n = 0; n < CAP; ++n)
-                        if (n < live) {
-                            const size_t at = (size_t)(row0 + n) * a.out + o;
-                            store_act(a.y, a.y_dt, at, acc[0][n] + (MODE == kFp8Down && a.shared ? load_act(a.shared, a.y_dt, at) : 0.0f));
-                        }
+                for (uint32_t n = 0; n < CAP; ++n) mid[(four * CAP + n) * 128u] = n & 1u ? sums[n >> 1].y : sums[n >> 1].x;
+                if (a.split > 1u && threadIdx.x == 0) mbar_arrive_expect_tx_addr(bars + kBarRecvFull, __popc(columns & ((1u << (live - 1u)) * 2u - 1u)) * a.split * 512u);
+                named_sync(4, kEpiWarps * 32u);
+                const uint32_t at = base + l.part + rank * own * 512u + row * 4u;
+#pragma unroll 1
+                for (uint32_t n = four; n < live; n += 2u) {
+                    const float v = mid[n * 128u] + mid[(CAP + n) * 128u];
+                    const uint32_t j = n / a.split, to = n - j * a.split;
+                    if (a.split > 1u) peer_store(peer_addr(at + j * 512u, to), v, peer_addr(bars + kBarRecvFull, to));
+                    else *reinterpret_cast<float*>(smem + (at - base) + j * 512u) = v;
+                }
             }
         }
     }
@@ -400,31 +550,38 @@ __global__ void __launch_bounds__(kThreads, CAP <= 64u ? 2 : 1) fp8_rows(const _
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, kCols);  // ahead of the wait for the other CTAs: they may be waiting for tensor memory themselves
+        __syncwarp();
     }
     if (a.split > 1u) {
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (MODE != kFp8GateUp) {
-            const uint32_t own = (CAP + a.split - 1u) / a.split, row = threadIdx.x & 127u, o = cluster * 128u + row;
-            const float* part = reinterpret_cast<const float*>(smem + l.part);
-            if (o < a.out)
-                for (uint32_t j = threadIdx.x >> 7; rank + j * a.split < live; j += 2u) {
-                    float v = 0.0f;
-                    for (uint32_t s = 0; s < a.split; ++s) v += part[(s * own + j) * 128u + row];
-                    const size_t at = (size_t)(row0 + rank + j * a.split) * a.out + o;
-                    store_act(a.y, a.y_dt, at, v + (MODE == kFp8Down && a.shared ? load_act(a.shared, a.y_dt, at) : 0.0f));
-                }
-        }
+        // no CTA leaves while another may still write to it (linear and down: what is written is counted on the barrier as well)
+        if (MODE == kFp8GateUp) cluster_arrive();
+        else cluster_arrive_relaxed();
     }
+    if (MODE != kFp8GateUp) {
+        if (a.split > 1u) fp8_wait<true>(bars + kBarRecvFull, 0, dead, a.err, kErrFullWait);
+        if (early) pdl_wait();
+        const uint32_t own = (CAP + a.split - 1u) / a.split, row = threadIdx.x & 127u, o = cluster * 128u + row;
+        const float* part = reinterpret_cast<const float*>(smem + l.part) + row;
+        if (o < a.out)
+#pragma unroll 1
+            for (uint32_t j = threadIdx.x >> 7; rank + j * a.split < live; j += kThreads / 128u) {
+                float v = 0.0f;
+#pragma unroll 1
+                for (uint32_t s = 0; s < a.split; ++s) v += part[(s * own + j) * 128u];
+                const size_t at = (size_t)(rank + j * a.split) * a.out + o;
+                if (MODE == kFp8Down && a.shared) v += load_act(a.shared, a.y_dt, at);
+                store_act(a.y, a.y_dt, at, v);
+            }
+        __syncwarp();
+    }
+    if (a.split > 1u) cluster_wait();
 }
 
 template <int MODE, uint32_t CAP, bool QUANT>
-cudaError_t launch_as(const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t row_tiles, uint32_t smem, bool overlap,
-                      cudaStream_t stream) {
+cudaError_t launch_as(const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     if (cudaError_t rc = allow_smem_once(ready, reinterpret_cast<const void*>(fp8_rows<MODE, CAP, QUANT>), 227u * 1024u)) return rc;
-    return launch_overlapped(fp8_rows<MODE, CAP, QUANT>, dim3(clusters * a.split, row_tiles), kThreads, smem, stream, overlap, a.split, maps, a);
+    return launch_overlapped(fp8_rows<MODE, CAP, QUANT>, dim3(clusters * a.split), kThreads, smem, stream, overlap, a.split, maps, a);
 }
 
 }  // namespace
@@ -434,28 +591,19 @@ uint32_t fp8_rows_smem(int mode, uint32_t cap, bool quantise, uint32_t slice_max
     return layout_of(mode, cap, quantise, slice_max, split, stages, experts, slots).total + 1024u;
 }
 
-cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t row_tiles,
-                            uint32_t smem, bool overlap, cudaStream_t stream) {
-    auto as = [&](auto m, auto c, auto q) {
-        return launch_as<decltype(m)::value, decltype(c)::value, decltype(q)::value>(maps, a, clusters, row_tiles, smem, overlap, stream);
-    };
-    using std::integral_constant;
-    constexpr auto no = std::false_type{};
-    constexpr auto yes = std::true_type{};
-    const integral_constant<uint32_t, 16> c16;
-    const integral_constant<uint32_t, 32> c32;
-    const integral_constant<uint32_t, 64> c64;
-    const integral_constant<uint32_t, 128> c128;
-    if (mode == kFp8GateUp) return cap == 16u ? as(integral_constant<int, kFp8GateUp>{}, c16, yes) : as(integral_constant<int, kFp8GateUp>{}, c32, yes);
-    if (mode == kFp8Down) return cap == 16u ? as(integral_constant<int, kFp8Down>{}, c16, no) : as(integral_constant<int, kFp8Down>{}, c32, no);
-    const integral_constant<int, kFp8Linear> lin;
-    if (a.x) return cap == 16u ? as(lin, c16, yes) : as(lin, c32, yes);
-    switch (cap) {
-        case 16: return as(lin, c16, no);
-        case 32: return as(lin, c32, no);
-        case 64: return as(lin, c64, no);
-        default: return as(lin, c128, no);
-    }
+cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap,
+                            cudaStream_t stream) {
+    if (mode == kFp8GateUp)
+        return cap == 16u ? launch_as<kFp8GateUp, 16, true>(maps, a, clusters, smem, overlap, stream)
+                          : launch_as<kFp8GateUp, 32, true>(maps, a, clusters, smem, overlap, stream);
+    if (mode == kFp8Down)
+        return cap == 16u ? launch_as<kFp8Down, 16, false>(maps, a, clusters, smem, overlap, stream)
+                          : launch_as<kFp8Down, 32, false>(maps, a, clusters, smem, overlap, stream);
+    if (a.x)
+        return cap == 16u ? launch_as<kFp8Linear, 16, true>(maps, a, clusters, smem, overlap, stream)
+                          : launch_as<kFp8Linear, 32, true>(maps, a, clusters, smem, overlap, stream);
+    return cap == 16u ? launch_as<kFp8Linear, 16, false>(maps, a, clusters, smem, overlap, stream)
+                      : launch_as<kFp8Linear, 32, false>(maps, a, clusters, smem, overlap, stream);
 }
 
 }  // namespace t3
