@@ -16,7 +16,13 @@ constexpr uint32_t kFp8SplitMax = 8;      // K slices of a tile: the portable cl
 // What a launch of the streaming kernel does (t3_fp8_rows.cu)
 enum Fp8Mode : int { kFp8Linear = 0, kFp8GateUp = 1, kFp8Down = 2 };
 
+// Shared memory of a streaming CTA: offsets from a 1024-byte boundary
+struct Fp8RowsLayout {
+    uint32_t rows, part, hid, red, sx, fetch, c, mask, list, chunks, slots, weight, bars, total;  // (the ring of weights at 0)
+};
+
 struct Fp8RowsArgs {
+    Fp8RowsLayout l;
     const void* x;         // [rows, in] in x_dt, quantised by the CTAs; or null: the rows are e4m3 already (the launch's row map)
     int x_dt;
     const float* x_scale;  // without x: [rows, in / 128] (down: the hidden rows', [experts used * cap, in / 128])
@@ -25,7 +31,6 @@ struct Fp8RowsArgs {
     void* y;               // [rows, out] in y_dt
     int y_dt;
     uint32_t split;        // K slices, CTAs of a cluster
-    uint32_t slice_max;    // 128-blocks of the largest slice (linear, gate|up)
     uint32_t stages;       // 128 x 128 weight tiles in flight a CTA
     uint32_t early;        // linear without x: the rows are the output of this call's launch before this one, which has waited for the weights
     // routed
@@ -45,9 +50,9 @@ struct Fp8Maps {
 };
 
 // `cap`: columns of a tile (rows of the call it serves): 16 or 32
-uint32_t fp8_rows_smem(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages, uint32_t experts,
-                       uint32_t slots);
-cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap,
+Fp8RowsLayout fp8_rows_layout(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages, uint32_t experts,
+                              uint32_t slots);
+cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, bool overlap,
                             cudaStream_t stream);
 
 // The linear past 32 rows (t3_fp8_gemm.cu)

@@ -21,22 +21,22 @@ constexpr uint32_t kTwo = 113u * 1024u, kOne = 227u * 1024u;
 constexpr uint32_t kStagesMost = 12;
 
 struct RowsPlan {
-    uint32_t cap, split, slice_max, stages, smem, per_sm;
+    uint32_t cap, split, slice_max, stages, per_sm;
     bool quantise;
+    Fp8RowsLayout layout;
 };
 
-// Weight tiles in flight: what fits beside the rest, two CTAs a multiprocessor where four tiles a CTA do
+// Weight tiles in flight: what fits beside the rest, two CTAs a multiprocessor where that leaves each three tiles (a stream of 16 KB tiles, 224 CTAs:
+// 5.0 TB/s with two in flight, 5.6 with three or more)
 bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots) {
     for (uint32_t per = 2u; per >= 1u; --per) {
-        const uint32_t room = per == 2u ? kTwo : kOne;
-        uint32_t stages = kStagesMost < units ? kStagesMost : units;
-        stages = stages < 2u ? 2u : stages;
-        while (stages > 2u && fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) --stages;
-        if (fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots) > room) continue;
-        if (per == 2u && stages < 4u && stages < units) continue;
-        p.stages = stages, p.per_sm = per;
-        p.smem = fp8_rows_smem(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots);
-        return true;
+        for (uint32_t stages = kStagesMost < units ? kStagesMost : units < 2u ? 2u : units; stages >= 2u; --stages) {
+            if (per == 2u && stages < 3u && stages < units) break;
+            const Fp8RowsLayout l = fp8_rows_layout(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots);
+            if (l.total > (per == 2u ? kTwo : kOne)) continue;
+            p.stages = stages, p.per_sm = per, p.layout = l;
+            return true;
+        }
     }
     return false;
 }
@@ -106,8 +106,8 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     p.clusters = tasks < most ? tasks : most;
     // down: one tile a cluster, as many slices as are resident at once
     s = 1;
-    for (uint32_t t = 2; t <= kFp8SplitMax; ++t)
-        if (hk * t <= resident(2, t)) s = t;
+    for (uint32_t t = 2; t <= kFp8SplitMax; ++t)  // (with room to spare: they are placed among gate|up's last CTAs, and a cluster that is left over is 20 us)
+        if (hk * t <= resident(2, t) * 7u / 8u) s = t;
     p.down.split = s, p.down.slice_max = 0;
     if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots)) return false;
     const size_t h = up256((size_t)p.used_max * cap * (size_t)b.inter);
@@ -201,8 +201,9 @@ int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, 
     if (p.quantise) a.x = x, a.x_dt = x_dtype;
     else a.x_scale = scale;
     a.rows = (uint32_t)rows, a.in = in, a.out = out, a.w_scale[0] = static_cast<const float*>(w_scale);
-    a.y = y, a.y_dt = y_dtype, a.split = p.split, a.slice_max = p.slice_max, a.stages = p.stages, a.early = ahead, a.err = device_error_word();
-    return status_of(launch_fp8_rows(kFp8Linear, p.cap, maps, a, div_up(out, 128u), p.smem, overlap, stream));
+    a.y = y, a.y_dt = y_dtype, a.split = p.split, a.stages = p.stages, a.early = ahead, a.err = device_error_word();
+    a.l = p.layout;
+    return status_of(launch_fp8_rows(kFp8Linear, p.cap, maps, a, div_up(out, 128u), overlap, stream));
 }
 
 size_t t3_moe_fp8_workspace_bytes(size_t rows, int topk, const t3_fp8_bank* bank) {
@@ -234,22 +235,22 @@ int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank,
     Fp8RowsArgs a = {};
     a.x = x, a.x_dt = x_dtype, a.rows = (uint32_t)rows, a.in = hidden, a.out = inter;
     a.w_scale[0] = static_cast<const float*>(bank->gate.scale), a.w_scale[1] = static_cast<const float*>(bank->up.scale);
-    a.split = p.up.split, a.slice_max = p.up.slice_max, a.stages = p.up.stages;
+    a.split = p.up.split, a.stages = p.up.stages, a.l = p.up.layout;
     a.inds = static_cast<const uint32_t*>(inds), a.scores = scores, a.score_dt = scores_dtype, a.topk = (uint32_t)topk, a.experts = experts;
     a.h = static_cast<uint8_t*>(workspace), a.h_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.h_scale);
     a.err = device_error_word();
     const bool overlap = launches_overlap();
     note_geometry(0, hidden, inter, experts, 8);
     count_launches(1);
-    if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, p.up.smem, overlap, static_cast<cudaStream_t>(stream)))
+    if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, overlap, static_cast<cudaStream_t>(stream)))
         return status_of(rc);
     Fp8RowsArgs d = a;
     d.x = nullptr, d.x_scale = a.h_scale, d.in = inter, d.out = hidden;
     d.w_scale[0] = static_cast<const float*>(bank->down.scale), d.w_scale[1] = nullptr;
-    d.split = p.down.split, d.slice_max = p.down.slice_max, d.stages = p.down.stages;
+    d.split = p.down.split, d.stages = p.down.stages, d.l = p.down.layout;
     d.shared = shared, d.y = y, d.y_dt = x_dtype;
     count_launches(1);
-    return status_of(launch_fp8_rows(kFp8Down, cap, down, d, hidden / 128u, p.down.smem, overlap, static_cast<cudaStream_t>(stream)));
+    return status_of(launch_fp8_rows(kFp8Down, cap, down, d, hidden / 128u, overlap, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -44,40 +44,7 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 // down: the most experts one of `split` slices of `used` experts' inputs touches
 __host__ __device__ constexpr uint32_t slice_experts(uint32_t used, uint32_t split) { return (used + split - 1u) / split + 1u; }
 
-// Shared memory of a CTA, offsets from a 1024-byte boundary
-struct Layout {
-    uint32_t ring, rows, part, hid, red, sx, fetch, c, mask, list, chunks, slots, weight, bars, total;
-};
-__host__ __device__ __forceinline__ Layout layout_of(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages,
-                                                     uint32_t experts, uint32_t slots) {
-    Layout l;
-    uint32_t at = 0;
-    auto take = [&](uint32_t bytes) {
-        const uint32_t o = at;
-        at += (bytes + 15u) & ~15u;
-        return o;
-    };
-    const uint32_t own = (cap + split - 1u) / split, used = experts < slots ? experts : slots;  // own: columns a CTA adds up
-    const bool gate_up = mode == kFp8GateUp, routed = mode != kFp8Linear, down = mode == kFp8Down;
-    l.ring = take(stages * (kTileBytes + (quantise ? 0u : cap * 128u)));
-    l.rows = take(quantise ? slice_max * cap * 128u : 0u);
-    l.part = take(split * own * (gate_up ? 1024u : 512u));
-    l.hid = take(gate_up ? own * 512u : 0u);
-    l.red = take(gate_up ? own * 16u : 0u);
-    l.sx = take(quantise ? slice_max * cap * 4u : 0u);
-    l.fetch = take(2u * kAhead * 33u * 4u);
-    l.c = take(kAcc * cap * 4u);
-    l.mask = take(routed ? experts * 4u : 0u);
-    l.list = take(routed ? used * 8u : 0u);
-    l.chunks = take(routed ? 256u : 0u);  // a word for each 32 experts
-    l.slots = take(down ? slots * 8u : 0u);
-    l.weight = take(down ? slice_experts(used, split) * cap * 4u : 0u);
-    l.bars = take(512u);
-    l.total = at;
-    return l;
-}
-
-// places in Layout::bars
+// places in Fp8RowsLayout::bars
 constexpr uint32_t kBarFull = 0, kBarEmpty = 8u * kStagesMax, kBarAccFull = 16u * kStagesMax, kBarAccEmpty = kBarAccFull + 8u * kAcc,
                    kBarRecvFull = kBarAccEmpty + 8u * kAcc, kBarRecvEmpty = kBarRecvFull + 8u, kWords = kBarRecvEmpty + 8u;
 static_assert(kWords + 16u <= 512u, "barriers and words");
@@ -92,16 +59,16 @@ struct Slot {
     }
 };
 
-// The experts in use, ascending, each with the rows that chose it (a bit a row); ids outside the bank are nobody's. Returns how many.
-// The routing is read past L1: with the kernel before this one still running, by its own wait complete, but not known to this CTA's cache.
-__device__ __forceinline__ uint32_t list_experts(const Fp8RowsArgs& a, uint32_t* mask, uint2* list, uint32_t* chunks, uint32_t* count) {
+// The experts in use, ascending, each with the rows that chose it (a bit a row); ids outside the bank are nobody's. id: the experts of the slots
+// threadIdx.x, + kThreads, .. (a number past the bank's where there is none). mask: zeros, before a __syncthreads. Returns how many.
+constexpr uint32_t kIds = (32u * 32u + kThreads - 1u) / kThreads;
+__device__ __forceinline__ uint32_t list_experts(const Fp8RowsArgs& a, const uint32_t (&id)[kIds], uint32_t* mask, uint2* list, uint32_t* chunks, uint32_t* count) {
     const uint32_t slots = a.rows * a.topk, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     if (slots <= 32u) {  // one warp, a slot a lane, against every other slot (a token's call: 1.5 us by the general way below)
         if (warp == 0) {
-            uint32_t e = lane < slots ? __ldcg(a.inds + lane) : kFull;
-            if (e >= a.experts) e = kFull;
+            const uint32_t e = id[0];
             uint32_t rows = 0, smaller = 0;
-            bool first = e != kFull;
+            bool first = e < a.experts;
 #pragma unroll 1
             for (uint32_t t = 0, row = 0, k = 0; t < slots; ++t) {
                 const uint32_t other = __shfl_sync(kFull, e, t);
@@ -123,14 +90,10 @@ __device__ __forceinline__ uint32_t list_experts(const Fp8RowsArgs& a, uint32_t*
         __syncthreads();
         return *count;
     }
-#pragma unroll 1
-    for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) mask[e] = 0u;
     __syncthreads();
-#pragma unroll 1
-    for (uint32_t s = threadIdx.x; s < slots; s += kThreads) {
-        const uint32_t e = __ldcg(a.inds + s);
-        if (e < a.experts) atomicOr(&mask[e], 1u << (s / a.topk));
-    }
+#pragma unroll
+    for (uint32_t i = 0; i < kIds; ++i)
+        if (id[i] < a.experts) atomicOr(&mask[id[i]], 1u << ((threadIdx.x + i * kThreads) / a.topk));
     __syncthreads();
     const uint32_t runs = (a.experts + 31u) / 32u;  // at most 64
     static_assert(kFp8ExpertsMax <= 64u * 32u, "two words a lane");
@@ -175,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
     constexpr uint32_t kOps = MODE == kFp8GateUp ? 2u : 1u;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
-    const Layout l = layout_of(MODE, CAP, QUANT, a.slice_max, a.split, a.stages, a.experts, a.rows * a.topk);
+    const Fp8RowsLayout& l = a.l;
     const uint32_t base = smem_addr(smem), bars = base + l.bars;
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + l.bars + kWords);  // dead, tensor memory, experts in use
     volatile uint32_t* dead = words;
@@ -219,11 +182,28 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
         pdl_trigger();
     }
 
+    // The routing, on its way while the rows are quantised. It is read past L1: in down the kernel before this one still runs, and what that one
+    // has waited for need not be known to this multiprocessor's cache.
+    uint32_t id[kIds];
+    if (MODE != kFp8Linear) {
+        const uint32_t slots = a.rows * a.topk;
+#pragma unroll
+        for (uint32_t i = 0; i < kIds; ++i) {
+            const uint32_t s = threadIdx.x + i * kThreads;
+            id[i] = s < slots ? __ldcg(a.inds + s) : kFull;
+            if (MODE == kFp8Down && s < slots) reinterpret_cast<float*>(smem + l.slots)[2u * s + 1u] = load_act_cg(a.scores, a.score_dt, s);
+        }
+        uint32_t* mask = reinterpret_cast<uint32_t*>(smem + l.mask);
+        if (slots > 32u)
+#pragma unroll 1
+            for (uint32_t e = threadIdx.x; e < a.experts; e += kThreads) mask[e] = 0u;
+    }
+
     if (QUANT) {
         // The rows' slice to e4m3, a warp a group, a lane's four values to their place in the swizzled tile. The groups come through the ring
         // (which has no weights yet), a share of it a warp: all of a warp's are on their way at once.
         const uint32_t q0 = kbs * rank / a.split, nb = kbs * (rank + 1u) / a.split - q0, groups = live * nb;
-        const uint32_t bytes = a.x_dt == kF32 ? 512u : 256u, room = a.stages * kTileBytes / kWarps / bytes, stage = base + l.ring + warp * room * bytes;
+        const uint32_t bytes = a.x_dt == kF32 ? 512u : 256u, room = a.stages * kTileBytes / kWarps / bytes, stage = base + warp * room * bytes;
         const uint8_t* x = static_cast<const uint8_t*>(a.x);
         uint32_t g = warp, n = g / nb, kb = g - n * nb;
         const uint32_t dn = kWarps / nb, dk = kWarps - dn * nb;
@@ -261,14 +241,18 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
         if (MODE == kFp8Linear) __syncthreads();  // (list_experts is one)
     }
     uint32_t used = 1;
+    if (MODE == kFp8Down)
+#pragma unroll
+        for (uint32_t i = 0; i < kIds; ++i)
+            if (threadIdx.x + i * kThreads < a.rows * a.topk) reinterpret_cast<uint32_t*>(smem + l.slots)[2u * (threadIdx.x + i * kThreads)] = id[i];
     if (MODE != kFp8Linear)
-        used = list_experts(a, reinterpret_cast<uint32_t*>(smem + l.mask), list, reinterpret_cast<uint32_t*>(smem + l.chunks), &words[2]);
+        used = list_experts(a, id, reinterpret_cast<uint32_t*>(smem + l.mask), list, reinterpret_cast<uint32_t*>(smem + l.chunks), &words[2]);
 
     // This CTA's units: of each of its tasks (a tile; gate|up: an expert's tile, of which a cluster takes several) `units` blocks. A unit
     // is (weight, 128-block of inputs, expert's place in the list, tile); they are walked by additions alone, since a division for
     // each cost the lone warps that walk them more than their waits.
     const uint32_t all = MODE == kFp8Down ? used * kbs : kbs;
-    const uint32_t k0 = (uint32_t)((uint64_t)all * rank / a.split), k1 = (uint32_t)((uint64_t)all * (rank + 1u) / a.split);
+    const uint32_t k0 = all * rank / a.split, k1 = all * (rank + 1u) / a.split;  // (a bank has at most 2^24 blocks)
     const uint32_t units = (k1 - k0) * kOps;
     const uint32_t tasks = MODE == kFp8GateUp ? used * tiles : tiles;
     const uint32_t mine = MODE == kFp8GateUp ? (tasks > cluster ? (tasks - cluster + clusters - 1u) / clusters : 0u) : 1u;
@@ -294,11 +278,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
     float* weight = reinterpret_cast<float*>(smem + l.weight);
     if (MODE == kFp8Down && units) {
         // what the router gave each row for each of this slice's experts, over all of the row's slots that name the expert
-        uint2* slots = reinterpret_cast<uint2*>(smem + l.slots);
-#pragma unroll 1
-        for (uint32_t s = threadIdx.x; s < a.rows * a.topk; s += kThreads)
-            slots[s] = make_uint2(__ldcg(a.inds + s), __float_as_uint(load_act_cg(a.scores, a.score_dt, s)));
-        __syncthreads();
+        const uint2* slots = reinterpret_cast<const uint2*>(smem + l.slots);
         const uint32_t n = (k1 - 1u) / kbs + 1u - entry0;
 #pragma unroll 1
         for (uint32_t i = threadIdx.x; i < n * CAP; i += kThreads) {
@@ -306,14 +286,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
             const uint32_t r = i % CAP;
             float v = 0.0f;
             if ((e.y >> r) & 1u)
-#pragma unroll 1
+#pragma unroll 2
                 for (uint32_t k = 0; k < a.topk; ++k)
                     if (slots[r * a.topk + k].x == e.x) v += __uint_as_float(slots[r * a.topk + k].y);
             weight[i] = v;
         }
         __syncthreads();
     }
-    if (a.split > 1u) {
+    if (a.split > 1u && warp != kTmaWarp) {  // (the copies need no other CTA)
         __syncwarp();
         cluster_wait();
     }
@@ -331,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 pdl_trigger();
             }
             const uint32_t slot = rows_only ? i - ahead : s.i;
-            const uint32_t full = bars + kBarFull + 8u * slot, at = base + l.ring + slot * kStageBytes;
+            const uint32_t full = bars + kBarFull + 8u * slot, at = base + slot * kStageBytes;
             if (!rows_only) fp8_wait(bars + kBarEmpty + 8u * slot, s.parity ^ 1u, dead, a.err, kErrEmptyWait);
             if (elect_one()) {
                 if (!rows_only) {
@@ -350,12 +330,16 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
             if (i >= ahead) step(r);
         }
         if (early && blocks == 0u) pdl_wait();
+        if (a.split > 1u) {
+            __syncwarp();
+            cluster_wait();
+        }
     } else if (warp == kMmaWarp) {
         Slot s, c;
         uint32_t k = 0;  // gate|up, QUANT: the block's place in the slice, each twice
 #pragma unroll 1
         for (uint32_t i = 0; i < blocks; ++i) {
-            const uint32_t at = base + l.ring + s.i * kStageBytes;
+            const uint32_t at = base + s.i * kStageBytes;
             const uint64_t ad = umma_desc(at), bd = umma_desc(QUANT ? base + l.rows + k / kOps * CAP * 128u : at + kTileBytes);
             if (++k == units) k = 0;
             fp8_wait(bars + kBarAccEmpty + 8u * c.i, c.parity ^ 1u, dead, a.err, kErrEmptyWait);
@@ -511,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                     if (lane == 0) red[4u * j + quarter] = most;
                 }
                 named_sync(2u + four, 128);
-                if (a.split > 1u && lane < a.split) peer_arrive(peer_addr(bars + kBarRecvEmpty, lane));  // ahead of the stores below: a release waits for them
+                // (ahead of the stores below, which a release waits for; after the last task nobody waits, and a late arrival could find its CTA gone)
+                if (a.split > 1u && lane < a.split && turn + 1u < mine) peer_arrive(peer_addr(bars + kBarRecvEmpty, lane));
                 uint32_t m = mine_of;
 #pragma unroll 1
                 for (uint32_t j = 0; j < count; ++j, m &= m - 1u) {
@@ -527,19 +512,21 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 next_task(t);
             } else {
                 // both fours' sums over the ring, once every block has been multiplied, and from there to the CTAs that add the slices up
-                float* mid = reinterpret_cast<float*>(smem + l.ring) + row;
+                float* mid = reinterpret_cast<float*>(smem) + row;
                 named_sync(4, kEpiWarps * 32u);
 #pragma unroll
                 for (uint32_t n = 0; n < CAP; ++n) mid[(four * CAP + n) * 128u] = n & 1u ? sums[n >> 1].y : sums[n >> 1].x;
                 if (a.split > 1u && threadIdx.x == 0) mbar_arrive_expect_tx_addr(bars + kBarRecvFull, __popc(columns & ((1u << (live - 1u)) * 2u - 1u)) * a.split * 512u);
                 named_sync(4, kEpiWarps * 32u);
                 const uint32_t at = base + l.part + rank * own * 512u + row * 4u;
-#pragma unroll 1
+                uint32_t j = 0, to = four;  // column n's place in the CTA it goes to
+#pragma unroll 2
                 for (uint32_t n = four; n < live; n += 2u) {
                     const float v = mid[n * 128u] + mid[(CAP + n) * 128u];
-                    const uint32_t j = n / a.split, to = n - j * a.split;
+                    while (to >= a.split) to -= a.split, ++j;
                     if (a.split > 1u) peer_store(peer_addr(at + j * 512u, to), v, peer_addr(bars + kBarRecvFull, to));
                     else *reinterpret_cast<float*>(smem + (at - base) + j * 512u) = v;
+                    to += 2u;
                 }
             }
         }
@@ -552,11 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
         tmem_dealloc(tmem, kCols);  // ahead of the wait for the other CTAs: they may be waiting for tensor memory themselves
         __syncwarp();
     }
-    if (a.split > 1u) {
-        // no CTA leaves while another may still write to it (linear and down: what is written is counted on the barrier as well)
-        if (MODE == kFp8GateUp) cluster_arrive();
-        else cluster_arrive_relaxed();
-    }
+    if (a.split > 1u) cluster_arrive_relaxed();  // no CTA leaves while another may still write to it
     if (MODE != kFp8GateUp) {
         if (a.split > 1u) fp8_wait<true>(bars + kBarRecvFull, 0, dead, a.err, kErrFullWait);
         if (early) pdl_wait();
@@ -578,32 +561,55 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
 }
 
 template <int MODE, uint32_t CAP, bool QUANT>
-cudaError_t launch_as(const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap, cudaStream_t stream) {
+cudaError_t launch_as(const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, bool overlap, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     if (cudaError_t rc = allow_smem_once(ready, reinterpret_cast<const void*>(fp8_rows<MODE, CAP, QUANT>), 227u * 1024u)) return rc;
-    return launch_overlapped(fp8_rows<MODE, CAP, QUANT>, dim3(clusters * a.split), kThreads, smem, stream, overlap, a.split, maps, a);
+    return launch_overlapped(fp8_rows<MODE, CAP, QUANT>, dim3(clusters * a.split), kThreads, a.l.total, stream, overlap, a.split, maps, a);
 }
 
 }  // namespace
 
-uint32_t fp8_rows_smem(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages, uint32_t experts,
-                       uint32_t slots) {
-    return layout_of(mode, cap, quantise, slice_max, split, stages, experts, slots).total + 1024u;
+Fp8RowsLayout fp8_rows_layout(int mode, uint32_t cap, bool quantise, uint32_t slice_max, uint32_t split, uint32_t stages, uint32_t experts,
+                              uint32_t slots) {
+    Fp8RowsLayout l;
+    uint32_t at = stages * (kTileBytes + (quantise ? 0u : cap * 128u));
+    auto take = [&](uint32_t bytes) {
+        const uint32_t o = at;
+        at += (bytes + 15u) & ~15u;
+        return o;
+    };
+    const uint32_t own = (cap + split - 1u) / split, used = experts < slots ? experts : slots;  // own: columns a CTA adds up
+    const bool gate_up = mode == kFp8GateUp, routed = mode != kFp8Linear, down = mode == kFp8Down;
+    l.rows = take(quantise ? slice_max * cap * 128u : 0u);
+    l.part = take(split * own * (gate_up ? 1024u : 512u));
+    l.hid = take(gate_up ? own * 512u : 0u);
+    l.red = take(gate_up ? own * 16u : 0u);
+    l.sx = take(quantise ? slice_max * cap * 4u : 0u);
+    l.fetch = take(2u * kAhead * 33u * 4u);
+    l.c = take(kAcc * cap * 4u);
+    l.mask = take(routed ? experts * 4u : 0u);
+    l.list = take(routed ? used * 8u : 0u);
+    l.chunks = take(routed ? 256u : 0u);  // a word for each 32 experts
+    l.slots = take(down ? slots * 8u : 0u);
+    l.weight = take(down ? slice_experts(used, split) * cap * 4u : 0u);
+    l.bars = take(512u);
+    l.total = at + 1024u;  // (and the way to the boundary)
+    return l;
 }
 
-cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, uint32_t smem, bool overlap,
+cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const Fp8RowsArgs& a, uint32_t clusters, bool overlap,
                             cudaStream_t stream) {
     if (mode == kFp8GateUp)
-        return cap == 16u ? launch_as<kFp8GateUp, 16, true>(maps, a, clusters, smem, overlap, stream)
-                          : launch_as<kFp8GateUp, 32, true>(maps, a, clusters, smem, overlap, stream);
+        return cap == 16u ? launch_as<kFp8GateUp, 16, true>(maps, a, clusters, overlap, stream)
+                          : launch_as<kFp8GateUp, 32, true>(maps, a, clusters, overlap, stream);
     if (mode == kFp8Down)
-        return cap == 16u ? launch_as<kFp8Down, 16, false>(maps, a, clusters, smem, overlap, stream)
-                          : launch_as<kFp8Down, 32, false>(maps, a, clusters, smem, overlap, stream);
+        return cap == 16u ? launch_as<kFp8Down, 16, false>(maps, a, clusters, overlap, stream)
+                          : launch_as<kFp8Down, 32, false>(maps, a, clusters, overlap, stream);
     if (a.x)
-        return cap == 16u ? launch_as<kFp8Linear, 16, true>(maps, a, clusters, smem, overlap, stream)
-                          : launch_as<kFp8Linear, 32, true>(maps, a, clusters, smem, overlap, stream);
-    return cap == 16u ? launch_as<kFp8Linear, 16, false>(maps, a, clusters, smem, overlap, stream)
-                      : launch_as<kFp8Linear, 32, false>(maps, a, clusters, smem, overlap, stream);
+        return cap == 16u ? launch_as<kFp8Linear, 16, true>(maps, a, clusters, overlap, stream)
+                          : launch_as<kFp8Linear, 32, true>(maps, a, clusters, overlap, stream);
+    return cap == 16u ? launch_as<kFp8Linear, 16, false>(maps, a, clusters, overlap, stream)
+                      : launch_as<kFp8Linear, 32, false>(maps, a, clusters, overlap, stream);
 }
 
 }  // namespace t3
