@@ -73,7 +73,8 @@ __device__ __forceinline__ float load_act_cg(const void* p, int dt, size_t i) {
 // Waits for a barrier phase; gives up after a while, or at once when any wait of the CTA has given up (`dead`): every role then
 // still walks to its end, on values nobody will use, and the error word says so. CLUSTER: what other CTAs of the cluster wrote
 // before their arrivals is visible after it. The loop is a call: these kernels' code comes from memory again for every launch, behind the
-// weights that have passed through L2, and what it does not hold it does not wait for.
+// weights that have passed through L2, and what it does not hold it does not wait for. (fp8_wait_here: the loop in place, for a caller
+// with so many registers in use that keeping them ready for a call costs more.)
 constexpr uint32_t kFp8Tries = 1u << 22;
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
     return done != 0u;
 }
 template <bool CLUSTER>
-__device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+__device__ __forceinline__ void fp8_wait_here(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kFp8Tries; ++i) {
         if (fp8_try<CLUSTER>(bar, parity)) return;
@@ -99,6 +100,10 @@ __device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volati
     }
     *dead = 1u;
     if (err) atomicOr(err, bit);
+}
+template <bool CLUSTER>
+__device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+    fp8_wait_here<CLUSTER>(bar, parity, dead, err, bit);
 }
 template <bool CLUSTER = false>
 __device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {

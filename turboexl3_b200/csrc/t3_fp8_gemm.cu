@@ -9,7 +9,7 @@
 // and 256 of f32 multiply-adds, so the tensor cores bound long calls (and the board's power limit). Calls of few tiles are cut along
 // K, a CTA of a cluster a slice; each CTA sends the others their share of the columns and adds up its own, in slice order.
 //
-// One persistent CTA a multiprocessor, ten warps: 0-7 epilogue (a quarter of the rows, half of the columns each), 8 TMA, 9 tcgen05.mma.
+// One persistent CTA a multiprocessor, twelve warps (two idle, for the registers' sake): 0-7 epilogue (a quarter of the rows, half of the columns each), 8 TMA, 9 tcgen05.mma.
 // The outputs leave through shared memory, a warp 128 bytes of 32 rows at a time, so that a row's bytes are stored together.
 #include "t3_fp8.cuh"
 #include "t3_fp8.h"
@@ -18,7 +18,11 @@
 namespace t3 {
 namespace {
 
-constexpr uint32_t kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr uint32_t kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 384;
+// A multiprocessor's registers by role: the epilogue's warps hold 128 sums a thread, and at the 168 registers an even split gives they spilled
+// (1820 cycles a block against 512 of tensor core)
+constexpr uint32_t kRegsEven = 168, kRegsEpi = 216, kRegsOther = 72;
+static_assert(256u * kRegsEpi + 128u * kRegsOther <= kThreads * kRegsEven && kThreads * kRegsEven <= 65536u, "what the block is launched with");
 constexpr uint32_t kStages = 4, kRowBytes = 128u * 128u, kOutBytes = kEpiWarps * 4096u;
 
 __host__ __device__ constexpr uint32_t stage_bytes(uint32_t n) { return kRowBytes + n * 128u; }
@@ -104,61 +108,65 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
         cluster_wait();
     }
 
-    if (warp == kTmaWarp) {
-        // early: the rows are quantised by the launch before this one, which has waited for what was there before the call; a ring of weights comes
-        // first, then the rows beside them
-        const uint32_t units = tiles > first ? (tiles - first + stride - 1u) / stride * (k1 - k0) : 0u;
-        const uint32_t ahead = a.early ? min(kStages, units) : 0u;
-        uint32_t slot = 0, parity = 1, t = first, kb = k0, rt = first, rkb = k0;  // the weights' place, and the rows'
-#pragma unroll 1
-        for (uint32_t i = 0; i < units + ahead; ++i) {
-            const bool rows_only = i >= ahead && i < 2u * ahead;
-            if (a.early && i == ahead) {
-                pdl_wait();
-                pdl_trigger();
-            }
-            const uint32_t s = rows_only ? i - ahead : slot, bar = full + 8u * s, at = base + s * kStageBytes;
-            if (!rows_only) fp8_wait(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
-            if (elect_one()) {
-                if (!rows_only) {
-                    mbar_arrive_expect_tx_addr(bar, kStageBytes);
-                    tma_load_2d(at + kRowBytes, &wmap, (int)(kb * 128u), (int)(t / row_tiles * N), bar);
+    if (warp >= kEpiWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (warp == kTmaWarp) {
+            // early: the rows are quantised by the launch before this one, which has waited for what was there before the call; a ring of weights comes
+            // first, then the rows beside them
+            const uint32_t units = tiles > first ? (tiles - first + stride - 1u) / stride * (k1 - k0) : 0u;
+            const uint32_t ahead = a.early ? min(kStages, units) : 0u;
+            uint32_t slot = 0, parity = 1, t = first, kb = k0, rt = first, rkb = k0;  // the weights' place, and the rows'
+    #pragma unroll 1
+            for (uint32_t i = 0; i < units + ahead; ++i) {
+                const bool rows_only = i >= ahead && i < 2u * ahead;
+                if (a.early && i == ahead) {
+                    pdl_wait();
+                    pdl_trigger();
                 }
-                if (i >= ahead) tma_load_2d(at, &xmap, (int)(rkb * 128u), (int)(rt % row_tiles * 128u), bar);
-            }
-            __syncwarp();
-            if (!rows_only) {
-                if (++slot == kStages) slot = 0, parity ^= 1u;
-                if (++kb == k1) kb = k0, t += stride;
-            }
-            if (i >= ahead && ++rkb == k1) rkb = k0, rt += stride;
-        }
-        if (a.early && units == 0u) pdl_wait();
-    } else if (warp == kMmaWarp) {
-        uint32_t slot = 0, parity = 0, acc = 0, acc_parity = 1;
-#pragma unroll 1
-        for (uint32_t t = first; t < tiles; t += stride) {
-#pragma unroll 1
-            for (uint32_t kb = k0; kb < k1; ++kb) {
-                const uint32_t at = base + slot * kStageBytes;
-                const uint64_t ad = umma_desc(at), bd = umma_desc(at + kRowBytes);
-                fp8_wait(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
-                fp8_wait(full + 8u * slot, parity, dead, a.err, kErrFullWait);
-                tc_fence_after();
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j)  // 32 inputs each
-                    if (elect_one()) umma_e4m3(tmem + acc * N, ad + 2u * j, bd + 2u * j, j, kIdesc);
+                const uint32_t s = rows_only ? i - ahead : slot, bar = full + 8u * s, at = base + s * kStageBytes;
+                if (!rows_only) fp8_wait_here<false>(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
                 if (elect_one()) {
-                    umma_commit(empty + 8u * slot);
-                    umma_commit(acc_full + 8u * acc);
+                    if (!rows_only) {
+                        mbar_arrive_expect_tx_addr(bar, kStageBytes);
+                        tma_load_2d(at + kRowBytes, &wmap, (int)(kb * 128u), (int)(t / row_tiles * N), bar);
+                    }
+                    if (i >= ahead) tma_load_2d(at, &xmap, (int)(rkb * 128u), (int)(rt % row_tiles * 128u), bar);
                 }
                 __syncwarp();
-                if (++slot == kStages) slot = 0, parity ^= 1u;
-                acc ^= 1u;
-                if (acc == 0u) acc_parity ^= 1u;
+                if (!rows_only) {
+                    if (++slot == kStages) slot = 0, parity ^= 1u;
+                    if (++kb == k1) kb = k0, t += stride;
+                }
+                if (i >= ahead && ++rkb == k1) rkb = k0, rt += stride;
+            }
+            if (a.early && units == 0u) pdl_wait();
+        } else if (warp == kMmaWarp) {
+            uint32_t slot = 0, parity = 0, acc = 0, acc_parity = 1;
+    #pragma unroll 1
+            for (uint32_t t = first; t < tiles; t += stride) {
+    #pragma unroll 1
+                for (uint32_t kb = k0; kb < k1; ++kb) {
+                    const uint32_t at = base + slot * kStageBytes;
+                    const uint64_t ad = umma_desc(at), bd = umma_desc(at + kRowBytes);
+                    fp8_wait_here<false>(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
+                    fp8_wait_here<false>(full + 8u * slot, parity, dead, a.err, kErrFullWait);
+                    tc_fence_after();
+    #pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j)  // 32 inputs each
+                        if (elect_one()) umma_e4m3(tmem + acc * N, ad + 2u * j, bd + 2u * j, j, kIdesc);
+                    if (elect_one()) {
+                        umma_commit(empty + 8u * slot);
+                        umma_commit(acc_full + 8u * acc);
+                    }
+                    __syncwarp();
+                    if (++slot == kStages) slot = 0, parity ^= 1u;
+                    acc ^= 1u;
+                    if (acc == 0u) acc_parity ^= 1u;
+                }
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
         const uint32_t quarter = warp & 3u, half = warp >> 2, buffer = outs + warp * 4096u;
         if (a.early) pdl_wait();
         uint32_t acc = 0, parity = 0;
@@ -181,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     if (kb + p >= k1) break;
                     const float c = sx[p] * sw[p];
                     if (kb + p + 2u < k1) sx[p] = __ldg(xs + kb + p + 2u), sw[p] = __ldg(ws + kb + p + 2u);
-                    fp8_wait(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
+                    fp8_wait_here<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
                     tc_fence_after();
                     const uint32_t from = tmem + acc * N + half * kMine + ((quarter * 32u) << 16);
 #pragma unroll
@@ -251,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
     }
     if (SPLIT) {
         cluster_arrive_relaxed();
-        fp8_wait<true>(recv, 0, dead, a.err, kErrFullWait);
+        fp8_wait_here<true>(recv, 0, dead, a.err, kErrFullWait);
         if (a.early) pdl_wait();
         const uint32_t width = N / split, row0 = first % row_tiles * 128u, col0 = first / row_tiles * N + rank * width;
         const float* p = reinterpret_cast<const float*>(smem + (part - base));
