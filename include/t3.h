@@ -351,7 +351,7 @@ int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, 
  * and up [experts, inter, hidden], down [experts, hidden, inter]; scales f32 [experts, out / 128, in / 128]; hidden and inter multiples of
  * 128, experts 1..T3_FP8_EXPERTS_MAX. inds i32 / u32 and scores (scores_dtype) [rows, topk], topk 1..32; an id outside the bank is nobody's and
  * adds nothing, whatever its score (a padded row's, or another rank's of an expert-parallel layer); an id may come twice. shared:
- * [rows, hidden] in x's dtype added before the one rounding, or null. y in x's dtype. Rows 1..T3_DECODE_ROWS_MAX, more:
+ * [rows, hidden] in x's dtype (on 16 bytes, like y) added before the one rounding, or null. y in x's dtype. Rows 1..T3_DECODE_ROWS_MAX, more:
  * Exl3EngineNotImplemented. Workspace (256-byte aligned): t3_moe_fp8_workspace_bytes. */
 #define T3_FP8_EXPERTS_MAX 2048
 typedef struct {

@@ -93,7 +93,7 @@ def test_moe_refusals():
     for bad in (dict(dt=3), dict(sdt=3)):
         assert _moe(**bad) == "BadExl3Dtype", bad
     for bad in (dict(bank=_bank(hidden=200)), dict(bank=_bank(inter=64)), dict(bank=_bank(experts=0)), dict(bank=_bank(experts=2049)),
-                dict(bank=_bank(experts=2048, hidden=1 << 20)), dict(rows=0), dict(topk=0), dict(topk=33), dict(x=FAKE + 8),
+                dict(bank=_bank(experts=2048, hidden=1 << 20)), dict(rows=0), dict(topk=0), dict(topk=33), dict(x=FAKE + 8), dict(y=FAKE + 8), dict(shared=FAKE + 8),
                 dict(bank=_bank(w=FAKE + 8))):
         assert _moe(**bad) == "BadExl3Shape", bad
     assert _moe(rows=33) == "Exl3EngineNotImplemented"

@@ -141,9 +141,10 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void peer_store(uint32_t addr, float v, uint32_t bar) {
     asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void peer_store4(uint32_t addr, float4 v, uint32_t bar) {  // 16 bytes, on a 16-byte boundary
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(__float_as_uint(v.x)),
-                 "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar)
+// `bytes` (a multiple of 16, both ends on 16 bytes) of this CTA's shared memory to another's, counted on the barrier there. What the copy reads was
+// written ahead of a proxy_fence. For more than a value or two a thread: a peer_store is a transaction a lane (64 KB of them took 3 to 5 us).
+__device__ __forceinline__ void peer_copy(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
 __device__ __forceinline__ void peer_arrive(uint32_t bar) {

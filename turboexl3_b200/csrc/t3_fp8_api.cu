@@ -220,7 +220,8 @@ int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank,
         if (!p->w || !p->scale) return T3_NULL_POINTER;
     if (!act_ok(x_dtype) || !act_ok(scores_dtype)) return T3_BAD_EXL3_DTYPE;
     if (!bank_shape_ok(*bank) || rows < 1 || topk < 1 || topk > T3_REDUCE_MAX_TOPK || !on16(x) || !on16(bank->gate.w) || !on16(bank->up.w) ||
-        !on16(bank->down.w))
+        !on16(bank->down.w) ||
+        !on16(y) || !on16(shared))
         return T3_BAD_EXL3_SHAPE;
     MoePlan p;
     if (rows > T3_DECODE_ROWS_MAX || !plan_moe(rows, topk, *bank, p)) return T3_ENGINE_NOT_IMPLEMENTED;

@@ -26,10 +26,12 @@ static_assert(256u * kRegsEpi + 128u * kRegsOther <= kThreads * kRegsEven && kTh
 constexpr uint32_t kStages = 4, kRowBytes = 128u * 128u, kOutBytes = kEpiWarps * 4096u;
 
 __host__ __device__ constexpr uint32_t stage_bytes(uint32_t n) { return kRowBytes + n * 128u; }
-// the slices' sums: [slice][row][columns of this CTA]
-__host__ __device__ constexpr uint32_t part_bytes(uint32_t n, bool split) { return split ? 128u * n * 4u : 0u; }
-constexpr uint32_t smem_bytes(uint32_t n, bool split) { return kStages * stage_bytes(n) + kOutBytes + part_bytes(n, split) + 256u + 1024u; }
+// the slices' sums: [slice][column of this CTA][row], a column's rows padded against bank conflicts of a lane a column
+constexpr uint32_t kPartRows = 132;
+__host__ __device__ constexpr uint32_t part_bytes(uint32_t n, bool split) { return split ? kPartRows * n * 4u : 0u; }
+constexpr uint32_t smem_bytes(uint32_t n, bool split) { return kStages * stage_bytes(n) + (split ? 0u : kOutBytes) + part_bytes(n, split) + 256u + 1024u; }
 static_assert(smem_bytes(256, false) <= 227u * 1024u && smem_bytes(128, true) <= 227u * 1024u, "shared memory of a CTA");
+static_assert(kPartRows * 128u * 4u <= kStages * stage_bytes(128), "a CTA's sums over its ring");
 
 // 16-bit or f32 outputs of 32 rows x 128 bytes from a warp's buffer: y at (first row, first column); rows and columns past the ends are left out
 __device__ __forceinline__ void store_rows(uint32_t buffer, void* y, int dt, size_t row0, uint32_t rows, uint32_t col0, uint32_t out, uint32_t lane) {
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
     constexpr uint32_t kStageBytes = stage_bytes(N), kIdesc = idesc_m128(N), kCols = 2u * N, kMine = N / 2u;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
-    const uint32_t base = smem_addr(smem), outs = base + kStages * kStageBytes, part = outs + kOutBytes, bars = part + part_bytes(N, SPLIT);
+    const uint32_t base = smem_addr(smem), outs = base + kStages * kStageBytes, part = outs + (SPLIT ? 0u : kOutBytes), bars = part + part_bytes(N, SPLIT);
     uint8_t* bars_at = smem + (bars - base);
     // full[kStages], empty[kStages], accumulator full[2], empty[2], sums received
     const uint32_t full = bars, empty = bars + 8u * kStages, acc_full = bars + 16u * kStages, acc_empty = acc_full + 16u, recv = acc_full + 32u;
@@ -192,14 +194,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     fp8_wait_here<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
                     tc_fence_after();
                     const uint32_t from = tmem + acc * N + half * kMine + ((quarter * 32u) << 16);
+                    // (the next sixteen columns on their way under the multiply-adds of these: 125 -> 115 us at 8192 rows 2048 -> 6144)
+                    uint32_t v[2][16];
+                    tmem_ld_32x16(from, v[0]);
 #pragma unroll
-                    for (uint32_t b = 0; b < kMine; b += 32u) {
-                        uint32_t v[32];
-                        tmem_ld_32x32(from + b, v);
+                    for (uint32_t b = 0; b < kMine; b += 16u) {
+                        tmem_ld_wait(v[(b >> 4) & 1u]);
+                        if (b + 16u < kMine) tmem_ld_32x16(from + b + 16u, v[((b >> 4) + 1u) & 1u]);
 #pragma unroll
-                        for (uint32_t j = 0; j < 32u; j += 2u) fma2(sums[(b + j) / 2u], v[j], v[j + 1u], c, c);
+                        for (uint32_t j = 0; j < 16u; j += 2u) fma2(sums[(b + j) / 2u], v[(b >> 4) & 1u][j], v[(b >> 4) & 1u][j + 1u], c, c);
                     }
-                    tc_fence_before();
+tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_addr(acc_empty + 8u * acc);
                     acc ^= 1u;
@@ -207,14 +212,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                 }
             }
             if (SPLIT) {
-                // this thread's columns, four at a time, to the CTAs whose they are: [slice][row][N / split]
-                const uint32_t width = N / split, row = quarter * 32u + lane;
-                if (threadIdx.x == 0) mbar_arrive_expect_tx_addr(recv, 128u * N * 4u);
+                // the sums over the ring, whose every block has been multiplied, and each CTA's columns to it by one copy
+                const uint32_t bytes = N / split * kPartRows * 4u;
+                const uint32_t at = base + (half * kMine * kPartRows + quarter * 32u + lane) * 4u;
 #pragma unroll
-                for (uint32_t n = 0; n < kMine; n += 4u) {
-                    const uint32_t col = half * kMine + n, to = col / width, at = part + ((rank * 128u + row) * width + (col - to * width)) * 4u;
-                    peer_store4(peer_addr(at, to), make_float4(sums[n / 2u].x, sums[n / 2u].y, sums[n / 2u + 1u].x, sums[n / 2u + 1u].y), peer_addr(recv, to));
-                }
+                for (uint32_t n = 0; n < kMine; ++n)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + n * kPartRows * 4u), "f"(n & 1u ? sums[n >> 1].y : sums[n >> 1].x) : "memory");
+                if (threadIdx.x == 0) mbar_arrive_expect_tx_addr(recv, split * bytes);
+                proxy_fence();
+                named_sync(1, kEpiWarps * 32u);
+                if (threadIdx.x < split) peer_copy(peer_addr(part + rank * bytes, threadIdx.x), base + threadIdx.x * bytes, bytes, peer_addr(recv, threadIdx.x));
                 continue;
             }
             const uint32_t rows = row0 < a.rows ? min(32u, a.rows - row0) : 0u;
@@ -263,13 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
         if (a.early) pdl_wait();
         const uint32_t width = N / split, row0 = first % row_tiles * 128u, col0 = first / row_tiles * N + rank * width;
         const float* p = reinterpret_cast<const float*>(smem + (part - base));
+        const uint32_t shift = 31u - __clz(width);  // (the slices are a power of two)
 #pragma unroll 1
         for (uint32_t i = threadIdx.x; i < 128u * width; i += kThreads) {
-            const uint32_t r = i / width, n = i - r * width;
+            const uint32_t r = i >> shift, n = i & (width - 1u);
             if (row0 + r >= a.rows || col0 + n >= a.out) continue;
             float v = 0.0f;
-#pragma unroll 1
-            for (uint32_t s = 0; s < split; ++s) v += p[s * 128u * width + i];
+#pragma unroll 4
+            for (uint32_t s = 0; s < split; ++s) v += p[(s * width + n) * kPartRows + r];
             store_act(a.y, a.y_dt, (size_t)(row0 + r) * a.out + col0 + n, v);
         }
         __syncwarp();

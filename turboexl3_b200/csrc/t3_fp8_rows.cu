@@ -511,22 +511,34 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 named_sync(2u + four, 128);  // (red is written again for the next task)
                 next_task(t);
             } else {
-                // both fours' sums over the ring, once every block has been multiplied, and from there to the CTAs that add the slices up
+                // Both fours' sums over the ring, once every block has been multiplied, in the order of the CTAs that add the slices up (column
+                // n: rank n mod split), and to each by one copy
                 float* mid = reinterpret_cast<float*>(smem) + row;
-                named_sync(4, kEpiWarps * 32u);
+                const uint32_t wrap = (a.split * own - 1u) * 128u;
+                auto put = [&](bool add) {
+                    uint32_t at = 0, to = 0;
 #pragma unroll
-                for (uint32_t n = 0; n < CAP; ++n) mid[(four * CAP + n) * 128u] = n & 1u ? sums[n >> 1].y : sums[n >> 1].x;
-                if (a.split > 1u && threadIdx.x == 0) mbar_arrive_expect_tx_addr(bars + kBarRecvFull, __popc(columns & ((1u << (live - 1u)) * 2u - 1u)) * a.split * 512u);
+                    for (uint32_t n = 0; n < CAP; ++n) {
+                        mid[at] = (n & 1u ? sums[n >> 1].y : sums[n >> 1].x) + (add ? mid[at] : 0.0f);
+                        at += own * 128u;
+                        if (++to == a.split) to = 0, at -= wrap;
+                    }
+                };
                 named_sync(4, kEpiWarps * 32u);
-                const uint32_t at = base + l.part + rank * own * 512u + row * 4u;
-                uint32_t j = 0, to = four;  // column n's place in the CTA it goes to
-#pragma unroll 2
-                for (uint32_t n = four; n < live; n += 2u) {
-                    const float v = mid[n * 128u] + mid[(CAP + n) * 128u];
-                    while (to >= a.split) to -= a.split, ++j;
-                    if (a.split > 1u) peer_store(peer_addr(at + j * 512u, to), v, peer_addr(bars + kBarRecvFull, to));
-                    else *reinterpret_cast<float*>(smem + (at - base) + j * 512u) = v;
-                    to += 2u;
+                if (four) put(false);
+                named_sync(4, kEpiWarps * 32u);
+                if (!four) {
+                    put(true);
+                    if (a.split > 1u) {
+                        proxy_fence();
+                        if (threadIdx.x == 0)
+                            mbar_arrive_expect_tx_addr(bars + kBarRecvFull, __popc(columns & ((1u << (live - 1u)) * 2u - 1u)) * a.split * 512u);
+                        named_sync(2, 128);
+                        const uint32_t to = threadIdx.x;
+                        if (to < a.split && to < live)
+                            peer_copy(peer_addr(base + l.part + rank * own * 512u, to), base + to * own * 512u, (live - to + a.split - 1u) / a.split * 512u,
+                                      peer_addr(bars + kBarRecvFull, to));
+                    }
                 }
             }
         }
@@ -543,18 +555,34 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
     if (MODE != kFp8GateUp) {
         if (a.split > 1u) fp8_wait<true>(bars + kBarRecvFull, 0, dead, a.err, kErrFullWait);
         if (early) pdl_wait();
-        const uint32_t own = (CAP + a.split - 1u) / a.split, row = threadIdx.x & 127u, o = cluster * 128u + row;
-        const float* part = reinterpret_cast<const float*>(smem + l.part) + row;
-        if (o < a.out)
+        // a lane four outputs of a column, a warp a column
+        const uint32_t own = (CAP + a.split - 1u) / a.split, o = cluster * 128u + 4u * lane;
+        const uint32_t part = base + (a.split > 1u ? l.part : 0u) + 16u * lane;
 #pragma unroll 1
-            for (uint32_t j = threadIdx.x >> 7; rank + j * a.split < live; j += kThreads / 128u) {
-                float v = 0.0f;
-#pragma unroll 1
-                for (uint32_t s = 0; s < a.split; ++s) v += part[(s * own + j) * 128u];
-                const size_t at = (size_t)(rank + j * a.split) * a.out + o;
-                if (MODE == kFp8Down && a.shared) v += load_act(a.shared, a.y_dt, at);
-                store_act(a.y, a.y_dt, at, v);
+        for (uint32_t j = warp; rank + j * a.split < live; j += kWarps) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+            for (uint32_t s = 0; s < a.split; ++s) {
+                float4 f;
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(part + (s * own + j) * 512u));
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
             }
+            const size_t at = (size_t)(rank + j * a.split) * a.out + o;
+            if (a.out % 4u == 0u) {
+                if (o >= a.out) continue;
+                if (MODE == kFp8Down && a.shared) {
+                    float f[4];
+                    load_act4(a.shared, a.y_dt, at, f);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) v[k] += f[k];
+                }
+                store_act4(a.y, a.y_dt, at, v);
+            } else {  // (a linear's)
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k)
+                    if (o + k < a.out) store_act(a.y, a.y_dt, at + k, v[k]);
+            }
+        }
         __syncwarp();
     }
     if (a.split > 1u) cluster_wait();
