@@ -61,6 +61,33 @@ def test_ties_masks_and_odd_values(dtype, scoring, bias, groups):
     close(got_s, want_s)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,group_topk,topk", [(64, 1, 1, 6), (64, 8, 3, 6), (8, 8, 5, 4), (60, 3, 2, 7), (1024, 2, 1, 16)])
+def test_picks_that_32_bits_cannot_tell_apart(scoring, experts, groups, group_topk, topk):
+    """Scores plus biases that differ by less than an f32 step of them, equal ones, and saturated scores: the order of the 64-bit sums."""
+    gen = torch.Generator().manual_seed(experts + groups)
+    x = torch.randint(-3, 4, (40, experts), generator=gen).float()
+    x[10:20] += 2.0 ** -22 * torch.randint(-2, 3, (10, experts), generator=gen)
+    x[20:25] = 30.0 + torch.randn(5, experts, generator=gen)
+    x[25:30] = -torch.finfo(torch.float32).max
+    x[27, ::5] = 1.0
+    b = torch.randint(0, 3, (experts,), generator=gen).float() * 0.25 + 2.0 ** -24 * torch.randint(-1, 2, (experts,), generator=gen)
+    got_i, got_s = t3.route(x.cuda(), topk, scoring, b.cuda(), groups, group_topk, True, 1.0)
+    want_i, want_s = ref.route(x, topk, scoring, b, groups, group_topk, True, 1.0)
+    assert torch.equal(got_i.cpu().long(), want_i)
+    close(got_s, want_s)
+
+
+def test_an_odd_bias_shows():
+    x = torch.randn(4, 32, generator=torch.Generator().manual_seed(1))
+    b = torch.zeros(32)
+    b[7], b[9], b[11] = math.nan, math.inf, -math.inf
+    for groups in (1, 4):
+        got_i, _ = t3.route(x.cuda(), 3, "sigmoid", b.cuda(), groups, min(groups, 2))
+        want_i, _ = ref.route(x, 3, "sigmoid", b, groups, min(groups, 2))
+        assert torch.equal(got_i.cpu().long(), want_i)
+
+
 def test_leading_shape_feeds_the_routed_layer():
     x = torch.randn(2, 3, 64, device="cuda")
     inds, scores = t3.route(x, 4)

@@ -13,49 +13,56 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kUnder = 4;  // groups a half warp has under way
 
+// the larger of each half of two words, as whole numbers of 16 bits
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads) fp8_quantize(const void* __restrict__ x, size_t groups, uint8_t* __restrict__ q, float* __restrict__ scale) {
-    pdl_trigger();
+    constexpr uint32_t kWords = DT == kF32 ? 8u : 4u;
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 15u;
+    pdl_trigger();
+    const uint32_t lane = threadIdx.x & 15u, half = 0xFFFFu << (threadIdx.x & 16u);
     const size_t step = (size_t)gridDim.x * (kThreads / 16u);
     for (size_t g0 = (size_t)blockIdx.x * (kThreads / 16u) + threadIdx.x / 16u; g0 < groups; g0 += step * kUnder) {
-        float v[kUnder][8];
+        uint32_t w[kUnder][kWords];
 #pragma unroll
         for (uint32_t j = 0; j < kUnder; ++j) {
             const size_t g = g0 + j * step;
             if (g >= groups) break;
-            const size_t at = g * 128u + lane * 8u;
-            if (DT == kF32) {
-                load_act4(x, DT, at, reinterpret_cast<float(&)[4]>(v[j][0]));
-                load_act4(x, DT, at + 4u, reinterpret_cast<float(&)[4]>(v[j][4]));
-            } else {
-                const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (g * 128u + lane * 8u) * (DT == kF32 ? 4u : 2u));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (DT == kF16) {
-                        const float2 f = unpack_half2(w[k]);
-                        v[j][2 * k] = f.x, v[j][2 * k + 1] = f.y;
-                    } else {
-                        v[j][2 * k] = __uint_as_float(w[k] << 16), v[j][2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-                    }
-                }
+            for (uint32_t k = 0; k < kWords / 4u; ++k) {
+                const uint4 u = __ldcs(from + k);
+                w[j][4u * k] = u.x, w[j][4u * k + 1u] = u.y, w[j][4u * k + 2u] = u.z, w[j][4u * k + 3u] = u.w;
             }
         }
 #pragma unroll
         for (uint32_t j = 0; j < kUnder; ++j) {
             const size_t g = g0 + j * step;
             if (g >= groups) break;  // (a half warp's lanes leave together)
+            // 16-bit magnitudes order as their bit patterns too, two to a word
             uint32_t most = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) most = max(most, magnitude(v[j][k]));
-            const uint32_t half = 0xFFFFu << (threadIdx.x & 16u);
+            for (uint32_t k = 0; k < kWords; ++k)
+                most = DT == kF32 ? max(most, w[j][k] & 0x7FFFFFFFu) : max_u16x2(most, w[j][k] & 0x7FFF7FFFu);
 #pragma unroll
-            for (uint32_t d = 8; d; d >>= 1) most = max(most, __shfl_xor_sync(half, most, d));
+            for (uint32_t d = 8; d; d >>= 1) {
+                const uint32_t other = __shfl_xor_sync(half, most, d);
+                most = DT == kF32 ? max(most, other) : max_u16x2(most, other);
+            }
+            if (DT == kBf16) most = max(most << 16, most & 0xFFFF0000u);
+            if (DT == kF16) most = __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(most & 0xFFFFu, most >> 16))));
             const float s = fp8_scale(most);
-            *reinterpret_cast<uint2*>(q + g * 128u + lane * 8u) = make_uint2(to_e4m3x4(reinterpret_cast<const float(&)[4]>(v[j][0]), s),
-                                                                             to_e4m3x4(reinterpret_cast<const float(&)[4]>(v[j][4]), s));
+            float v[2][4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                float2 f;
+                if (DT == kF32) f = make_float2(__uint_as_float(w[j][2u * k % kWords]), __uint_as_float(w[j][(2u * k + 1u) % kWords]));
+                else if (DT == kF16) f = unpack_half2(w[j][k]);
+                else f = make_float2(__uint_as_float(w[j][k] << 16), __uint_as_float(w[j][k] & 0xFFFF0000u));
+                v[k >> 1][2u * (k & 1u)] = f.x, v[k >> 1][2u * (k & 1u) + 1u] = f.y;
+            }
+            *reinterpret_cast<uint2*>(q + g * 128u + lane * 8u) = make_uint2(to_e4m3x4(v[0], s), to_e4m3x4(v[1], s));
             if (lane == 0) scale[g] = s;
         }
     }
@@ -66,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize(const void* __restrict_
 cudaError_t launch_fp8_quantize(const void* x, int dt, size_t rows, uint32_t in, uint8_t* q, float* scale, bool overlap, cudaStream_t stream) {
     const size_t groups = rows * (in / 128u), per = kThreads / 16u;
     size_t blocks = (groups + per - 1u) / per;
-    const size_t most = 148u * 8u;  // eight of 256 threads fill a multiprocessor
+    const size_t most = (size_t)multiprocessors() * 16u;
     if (blocks > most) blocks = most;
     const dim3 grid((unsigned)blocks);
     if (dt == kF32) return launch_overlapped(fp8_quantize<kF32>, grid, kThreads, 0, stream, overlap, 1, x, groups, q, scale);
