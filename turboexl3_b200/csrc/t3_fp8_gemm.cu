@@ -23,15 +23,17 @@ constexpr uint32_t kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 384;
 // (1820 cycles a block against 512 of tensor core)
 constexpr uint32_t kRegsEven = 168, kRegsEpi = 216, kRegsOther = 72;
 static_assert(256u * kRegsEpi + 128u * kRegsOther <= kThreads * kRegsEven && kThreads * kRegsEven <= 65536u, "what the block is launched with");
-constexpr uint32_t kStages = 4, kRowBytes = 128u * 128u, kOutBytes = kEpiWarps * 4096u;
+constexpr uint32_t kRowBytes = 128u * 128u, kOutBytes = kEpiWarps * 4096u;
+// blocks in flight; tiles of 64 outputs serve calls of few tiles, whose slices are short: all of a slice at once
+__host__ __device__ constexpr uint32_t stages_of(uint32_t n) { return n == 64u ? 8u : 4u; }
 
 __host__ __device__ constexpr uint32_t stage_bytes(uint32_t n) { return kRowBytes + n * 128u; }
 // the slices' sums: [slice][column of this CTA][row], a column's rows padded against bank conflicts of a lane a column
 constexpr uint32_t kPartRows = 132;
 __host__ __device__ constexpr uint32_t part_bytes(uint32_t n, bool split) { return split ? kPartRows * n * 4u : 0u; }
-constexpr uint32_t smem_bytes(uint32_t n, bool split) { return kStages * stage_bytes(n) + (split ? 0u : kOutBytes) + part_bytes(n, split) + 256u + 1024u; }
-static_assert(smem_bytes(256, false) <= 227u * 1024u && smem_bytes(128, true) <= 227u * 1024u, "shared memory of a CTA");
-static_assert(kPartRows * 128u * 4u <= kStages * stage_bytes(128), "a CTA's sums over its ring");
+constexpr uint32_t smem_bytes(uint32_t n, bool split) { return stages_of(n) * stage_bytes(n) + (split ? 0u : kOutBytes) + part_bytes(n, split) + 256u + 1024u; }
+static_assert(smem_bytes(256, false) <= 227u * 1024u && smem_bytes(128, true) <= 227u * 1024u && smem_bytes(64, true) <= 227u * 1024u, "shared memory of a CTA");
+static_assert(kPartRows * 128u * 4u <= stages_of(128) * stage_bytes(128), "a CTA's sums over its ring");
 
 // 16-bit or f32 outputs of 32 rows x 128 bytes from a warp's buffer: y at (first row, first column); rows and columns past the ends are left out
 __device__ __forceinline__ void store_rows(uint32_t buffer, void* y, int dt, size_t row0, uint32_t rows, uint32_t col0, uint32_t out, uint32_t lane) {
@@ -69,7 +71,7 @@ __device__ __forceinline__ uint32_t pack_as(float a, float b, int dt) {
 template <uint32_t N, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                                                          const __grid_constant__ Fp8GemmArgs a) {
-    constexpr uint32_t kStageBytes = stage_bytes(N), kIdesc = idesc_m128(N), kCols = 2u * N, kMine = N / 2u;
+    constexpr uint32_t kStages = stages_of(N), kStageBytes = stage_bytes(N), kIdesc = idesc_m128(N), kCols = 2u * N, kMine = N / 2u;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
     const uint32_t base = smem_addr(smem), outs = base + kStages * kStageBytes, part = outs + (SPLIT ? 0u : kOutBytes), bars = part + part_bytes(N, SPLIT);
@@ -299,24 +301,31 @@ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
 Fp8GemmPlan plan_fp8_gemm(uint32_t rows, uint32_t in, uint32_t out) {
     const uint32_t sms = multiprocessors(), kbs = in / 128u, row_tiles = div_up(rows, 128u);
-    const uint32_t wide = row_tiles * div_up(out, 256u), narrow = row_tiles * div_up(out, 128u);
+    const uint32_t wide = row_tiles * div_up(out, 256u), narrow = row_tiles * div_up(out, 128u), slim = row_tiles * div_up(out, 64u);
     Fp8GemmPlan p = {256u, 1u, 0u};
-    // Few tiles: narrow ones, cut along K as long as all clusters are resident at once (one CTA a multiprocessor), four blocks a slice at least
+    // Few tiles: narrow ones, cut along K as long as all clusters are resident at once (one CTA a multiprocessor), four blocks a slice at least.
+    // What the CTAs of a cluster send each other is 64 KB a CTA from tiles of 128 outputs, half as much from tiles of 64.
     static const uint32_t resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    auto slices = [&](uint32_t tiles) {
+        uint32_t s = 1;
+        while (s < 8u && kbs >= s * 8u && tiles <= resident[s * 2u] * sms / 148u) s *= 2u;
+        return s;
+    };
     if (narrow * 2u <= sms) {
-        p.n = 128u;
-        while (p.split < 8u && kbs >= p.split * 8u && narrow <= resident[p.split * 2u] * sms / 148u) p.split *= 2u;
+        p.n = slices(slim) > 1u ? 64u : 128u;
+        p.split = slices(p.n == 64u ? slim : narrow);
     } else if (div_up(narrow, sms) * 5u < div_up(wide, sms) * 8u) {
         // a round of narrow tiles takes some five eighths of a round of wide ones
         p.n = 128u;
     }
-    const uint32_t tiles = p.n == 256u ? wide : narrow;
+    const uint32_t tiles = p.n == 256u ? wide : p.n == 128u ? narrow : slim;
     p.grid = p.split > 1u ? tiles * p.split : tiles < sms ? tiles : sms;
     return p;
 }
 
 cudaError_t launch_fp8_gemm(const CUtensorMap& w, const CUtensorMap& x, const Fp8GemmArgs& a, const Fp8GemmPlan& p, bool overlap, cudaStream_t stream) {
     if (p.n == 256u) return launch_as<256, false>(w, x, a, p.grid, overlap, stream);
+    if (p.n == 64u) return launch_as<64, true>(w, x, a, p.grid, overlap, stream);
     if (p.split > 1u) return launch_as<128, true>(w, x, a, p.grid, overlap, stream);
     return launch_as<128, false>(w, x, a, p.grid, overlap, stream);
 }
