@@ -18,6 +18,8 @@ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
 // Shared memory a CTA may take: where two fit a multiprocessor (228 KB, 1 KB a CTA reserved), and one
 constexpr uint32_t kTwo = 113u * 1024u, kOne = 227u * 1024u;
+constexpr uint32_t kHalfMore = 115u * 1024u;  // no second CTA that takes as much fits beside it; one of up to 106 KB does beside kBeside
+constexpr uint32_t kBeside = 122u * 1024u;
 constexpr uint32_t kStagesMost = 12;
 
 struct RowsPlan {
@@ -26,22 +28,38 @@ struct RowsPlan {
     Fp8RowsLayout layout;
 };
 
-// Weight tiles in flight: what fits beside the rest, two CTAs a multiprocessor where that leaves each three tiles (a stream of 16 KB tiles, 224 CTAs:
-// 5.0 TB/s with two in flight, 5.6 with three or more)
-bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots) {
-    for (uint32_t per = 2u; per >= 1u; --per) {
+// resident CTAs of two a multiprocessor by cluster size, and of one (clusters lie inside a group of multiprocessors)
+uint32_t resident(uint32_t per_sm, uint32_t split) {
+    static const uint32_t two[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264}, one[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+    return (per_sm == 2u ? two[split] : one[split]) * multiprocessors() / 148u;
+}
+
+// the most slices, of at most `most`, whose CTAs all have a multiprocessor to themselves
+uint32_t slices_alone(uint32_t tiles, uint32_t most) {
+    uint32_t s = 1;
+    for (uint32_t t = 2; t <= kFp8SplitMax && t <= most; ++t)
+        if (tiles * t <= resident(1, t)) s = t;
+    return s;
+}
+
+// Weight tiles in flight: what fits beside the rest. pair: two CTAs a multiprocessor where that leaves each three tiles (a stream of 16 KB tiles, 224
+// CTAs: 5.0 TB/s with two in flight, 5.6 with three or more). Else up to `room` bytes, and at least what keeps a second one of its kind from the
+// multiprocessor: the hardware doubles up CTAs while other multiprocessors are empty, and the late ones set the launch's duration.
+bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots, bool pair, uint32_t room = kOne) {
+    for (uint32_t per = pair ? 2u : 1u; per >= 1u; --per) {
         for (uint32_t stages = kStagesMost < units ? kStagesMost : units < 2u ? 2u : units; stages >= 2u; --stages) {
             if (per == 2u && stages < 3u && stages < units) break;
             const Fp8RowsLayout l = fp8_rows_layout(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots);
-            if (l.total > (per == 2u ? kTwo : kOne)) continue;
+            if (l.total > (per == 2u ? kTwo : room)) continue;
             p.stages = stages, p.per_sm = per, p.layout = l;
+            if (!pair && p.layout.total < kHalfMore) p.layout.total = kHalfMore;
             return true;
         }
     }
     return false;
 }
 
-constexpr uint32_t kFusedGroups = 64;  // groups of 128 a CTA quantises itself
+constexpr uint32_t kFusedGroups = 128;  // groups of 128 a CTA quantises itself, of up to 16 rows: past that a launch ahead is quicker
 
 // K slices: what leaves the fullest multiprocessor the fewest 128-blocks, counting a CTA's fixed part as three of them
 uint32_t pick_slices(uint32_t tiles, uint32_t kbs) {
@@ -59,9 +77,16 @@ bool plan_linear(size_t rows, uint32_t in, uint32_t out, bool given, RowsPlan& p
     p.cap = rows <= 16u ? 16u : 32u;
     const uint32_t kbs = in / 128u, tiles = div_up(out, 128u);
     p.split = tiles >= multiprocessors() ? 1u : pick_slices(tiles, kbs);
+    // Long slices, and rows past 16, have their CTAs a multiprocessor each (16384 -> 7168 at one row 33 -> 24 us, at 29 rows 31 -> 27; 2048 -> 6144
+    // at 29 rows 11.1 -> 9.9); else two share one (7168 -> 4096 at 8 rows 11.4 -> 10.5).
+    bool pair = true;
+    if (tiles <= resident(1, 1)) {
+        const uint32_t s = slices_alone(tiles, kbs);
+        if (p.cap == 32u || div_up(kbs, s) >= 32u) pair = false, p.split = s;
+    }
     p.slice_max = div_up(kbs, p.split);
-    p.quantise = !given && (uint32_t)rows * p.slice_max <= kFusedGroups;
-    return fit(kFp8Linear, p, p.slice_max, 0, 0);
+    p.quantise = !given && p.cap == 16u && (uint32_t)rows * p.slice_max <= kFusedGroups;
+    return fit(kFp8Linear, p, p.slice_max, 0, 0, pair);
 }
 
 struct LinearWs {
@@ -84,24 +109,25 @@ struct MoePlan {
     size_t h_scale, total;
 };
 
-// resident CTAs of two a multiprocessor by cluster size, and of one (clusters lie inside a group of multiprocessors)
-uint32_t resident(uint32_t per_sm, uint32_t split) {
-    static const uint32_t two[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264}, one[9] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
-    return (per_sm == 2u ? two[split] : one[split]) * multiprocessors() / 148u;
-}
-
 bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     const uint32_t cap = rows <= 16u ? 16u : 32u, slots = (uint32_t)rows * (uint32_t)topk;
     const uint32_t hk = (uint32_t)b.hidden / 128u, ik = (uint32_t)b.inter / 128u;
     p.used_max = (uint32_t)b.experts < slots ? (uint32_t)b.experts : slots;
     p.up.cap = p.down.cap = cap;
     p.up.quantise = true, p.down.quantise = false;
-    // gate|up: four slices, or the eight that still are resident at once; as many as leave the quantised rows' slice room for weights
+    // gate|up. Few tasks: a CTA a multiprocessor, as many slices as that leaves, and room beside it for down's, which start on their weights while
+    // these finish (one row of 512 experts of 2048 x 512: 15.8 -> 13.2 us). Else four slices, two CTAs a multiprocessor. As many slices in
+    // any case as leave the quantised rows' slice room for weights.
     const uint32_t tasks = p.used_max * ik;
-    uint32_t s = 1;
-    while (s < kFp8SplitMax && s * 2u <= hk && (s < 4u || tasks * s * 2u <= resident(2, s * 2u) || div_up(hk, s) * cap * 128u > 32u * 1024u)) s *= 2u;
+    auto too_long = [&](uint32_t t) { return div_up(hk, t) * cap * 128u > 32u * 1024u; };
+    uint32_t s = tasks <= resident(1, 1) ? slices_alone(tasks, hk) : 1u;
+    const bool pair = tasks > resident(1, 1) || too_long(s);
+    if (pair)
+        for (s = 1; s < kFp8SplitMax && s * 2u <= hk && (s < 4u || too_long(s));) s *= 2u;
     p.up.split = s, p.up.slice_max = div_up(hk, s);
-    if (!fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots)) return false;
+    if (!fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots, pair, pair ? kOne : kBeside) &&
+        !fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots, true))
+        return false;
     const uint32_t most = resident(p.up.per_sm, s) / s;
     p.clusters = tasks < most ? tasks : most;
     // down: one tile a cluster, as many slices as are resident at once
@@ -109,7 +135,7 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     for (uint32_t t = 2; t <= kFp8SplitMax; ++t)  // (with room to spare: they are placed among gate|up's last CTAs, and a cluster that is left over is 20 us)
         if (hk * t <= resident(2, t) * 7u / 8u) s = t;
     p.down.split = s, p.down.slice_max = 0;
-    if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots)) return false;
+    if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots, true)) return false;
     const size_t h = up256((size_t)p.used_max * cap * (size_t)b.inter);
     p.h_scale = h;
     p.total = h + up256((size_t)p.used_max * cap * ik * 4u);

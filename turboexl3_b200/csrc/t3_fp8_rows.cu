@@ -633,9 +633,7 @@ cudaError_t launch_fp8_rows(int mode, uint32_t cap, const Fp8Maps& maps, const F
     if (mode == kFp8Down)
         return cap == 16u ? launch_as<kFp8Down, 16, false>(maps, a, clusters, overlap, stream)
                           : launch_as<kFp8Down, 32, false>(maps, a, clusters, overlap, stream);
-    if (a.x)
-        return cap == 16u ? launch_as<kFp8Linear, 16, true>(maps, a, clusters, overlap, stream)
-                          : launch_as<kFp8Linear, 32, true>(maps, a, clusters, overlap, stream);
+    if (a.x) return launch_as<kFp8Linear, 16, true>(maps, a, clusters, overlap, stream);
     return cap == 16u ? launch_as<kFp8Linear, 16, false>(maps, a, clusters, overlap, stream)
                       : launch_as<kFp8Linear, 32, false>(maps, a, clusters, overlap, stream);
 }
