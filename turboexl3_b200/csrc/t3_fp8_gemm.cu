@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
 #pragma unroll
                         for (uint32_t j = 0; j < 16u; j += 2u) fma2(sums[(b + j) / 2u], v[(b >> 4) & 1u][j], v[(b >> 4) & 1u][j + 1u], c, c);
                     }
-tc_fence_before();
+                    tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_addr(acc_empty + 8u * acc);
                     acc ^= 1u;
@@ -302,21 +302,22 @@ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 Fp8GemmPlan plan_fp8_gemm(uint32_t rows, uint32_t in, uint32_t out) {
     const uint32_t sms = multiprocessors(), kbs = in / 128u, row_tiles = div_up(rows, 128u);
     const uint32_t wide = row_tiles * div_up(out, 256u), narrow = row_tiles * div_up(out, 128u), slim = row_tiles * div_up(out, 64u);
-    Fp8GemmPlan p = {256u, 1u, 0u};
-    // Few tiles: narrow ones, cut along K as long as all clusters are resident at once (one CTA a multiprocessor), four blocks a slice at least.
-    // What the CTAs of a cluster send each other is 64 KB a CTA from tiles of 128 outputs, half as much from tiles of 64.
-    static const uint32_t resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
-    auto slices = [&](uint32_t tiles) {
-        uint32_t s = 1;
-        while (s < 8u && kbs >= s * 8u && tiles <= resident[s * 2u] * sms / 148u) s *= 2u;
-        return s;
+    // What a tile costs, in hundreds of cycles: its blocks, as they measured in long calls (at the power limit a tile of half the outputs is no twice as
+    // quick), the outputs, and a slice's exchange.
+    auto cost = [&](uint32_t tiles, uint32_t at_once, uint32_t blocks, uint32_t block, uint32_t fixed) {
+        return div_up(tiles, at_once) * (blocks * block + fixed);
     };
-    if (narrow * 2u <= sms) {
-        p.n = slices(slim) > 1u ? 64u : 128u;
-        p.split = slices(p.n == 64u ? slim : narrow);
-    } else if (div_up(narrow, sms) * 5u < div_up(wide, sms) * 8u) {
-        // a round of narrow tiles takes some five eighths of a round of wide ones
-        p.n = 128u;
+    Fp8GemmPlan p = {256u, 1u, 0u};
+    uint32_t best = cost(wide, sms, kbs, 7u, 40u);
+    uint32_t c = cost(narrow, sms, kbs, 6u, 30u);
+    if (c < best) best = c, p.n = 128u;
+    // Few tiles may be cut along K, as long as all clusters are resident at once (one CTA a multiprocessor). What the CTAs of a cluster send each
+    // other is 64 KB a CTA from narrow tiles, half as much from slim ones.
+    static const uint32_t resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    for (uint32_t s = 2; s <= 8u && s <= kbs; s *= 2u) {
+        const uint32_t at_once = resident[s] * sms / 148u;
+        if (narrow <= at_once && (c = cost(narrow, at_once, div_up(kbs, s), 6u, 110u)) < best) best = c, p.n = 128u, p.split = s;
+        if (slim <= at_once && (c = cost(slim, at_once, div_up(kbs, s), 5u, 80u)) < best) best = c, p.n = 64u, p.split = s;
     }
     const uint32_t tiles = p.n == 256u ? wide : p.n == 128u ? narrow : slim;
     p.grid = p.split > 1u ? tiles * p.split : tiles < sms ? tiles : sms;
