@@ -118,3 +118,27 @@ def test_python_refusals():
         t3.route(logits, 4, "tanh")
     with pytest.raises(t3.Exl3Error, match="BadExl3Dtype"):
         t3.linear_fp8(x, w, s, out_dtype=torch.int8)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 16, 17, 32])
+@pytest.mark.parametrize("width", [128, 1024, 7168, 16384, 131072, 1 << 20])
+def test_every_width_has_a_plan(rows, width):
+    """Where rows are quantised ahead, a call with a byte too little gets past the plan and is refused for the workspace."""
+    L = t3.lib()
+    for out in (1, 128, 576, 1000):
+        need = L.t3_linear_fp8_workspace_bytes(rows, width, out, 2)
+        if need:
+            assert need >= rows * (width + width // 32)
+            assert _linear(rows=rows, width=width, out=out, work_bytes=need - 1) == "WorkspaceTooSmall"
+
+
+@pytest.mark.parametrize("hidden", [128, 1024, 7168, 32768])
+@pytest.mark.parametrize("inter", [128, 2048, 16384])
+def test_every_layer_has_a_plan(hidden, inter):
+    L = t3.lib()
+    for experts in (1, 8, 512, 2048):
+        for rows in (1, 16, 17, 32):
+            for topk in (1, 8, 32):
+                if experts * max(hidden, inter) < 1 << 31:
+                    b = _bank(experts, hidden, inter)
+                    assert L.t3_moe_fp8_workspace_bytes(rows, topk, C.byref(b)) > 0

@@ -74,7 +74,7 @@ def test_quantize_of_an_infinity_or_nan_is_its_groups_alone(bad):
 # ---- the linear ----
 
 @pytest.mark.parametrize("rows,width,out,dtype", [
-    (1, 128, 1, torch.bfloat16), (1, 2048, 2048, torch.bfloat16), (2, 256, 17, torch.float16), (7, 1536, 576, torch.float32),
+    (1, 128, 1, torch.bfloat16), (1, 2048, 2048, torch.bfloat16), (1, 131072, 128, torch.bfloat16), (2, 256, 17, torch.float16), (7, 1536, 576, torch.float32),
     (16, 640, 255, torch.bfloat16), (17, 1024, 384, torch.float16), (29, 16384, 256, torch.bfloat16), (32, 384, 4096, torch.float32),
     (33, 512, 130, torch.bfloat16), (64, 2048, 128, torch.float16), (65, 896, 640, torch.float32), (128, 256, 1000, torch.bfloat16),
     (129, 7168, 576, torch.bfloat16), (300, 640, 333, torch.float32), (1000, 384, 1408, torch.float16), (2050, 128, 2048, torch.bfloat16),

@@ -86,6 +86,8 @@ bool plan_linear(size_t rows, uint32_t in, uint32_t out, bool given, RowsPlan& p
     }
     p.slice_max = div_up(kbs, p.split);
     p.quantise = !given && p.cap == 16u && (uint32_t)rows * p.slice_max <= kFusedGroups;
+    if (fit(kFp8Linear, p, p.slice_max, 0, 0, pair)) return true;
+    p.quantise = false;  // (the quantised rows of a slice of a hundred blocks leave no room for weights)
     return fit(kFp8Linear, p, p.slice_max, 0, 0, pair);
 }
 

@@ -95,14 +95,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
         mbar_init_fence();
     } else if (warp == kTmaWarp) {
         if (lane == 0) prefetch_map(&wmap), prefetch_map(&xmap);
-    } else if (warp == kMmaWarp) {
+    }
+    if (SPLIT) {  // (ahead of the allocation: no CTA waits, holding tensor memory, for one that waits for some)
+        __syncwarp();
+        cluster_arrive();
+    }
+    if (warp == kMmaWarp) {
         tmem_alloc(&words[1], kCols);
         tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = words[1];
-    if (SPLIT) cluster_arrive();
     if (!a.early) {
         pdl_wait();
         pdl_trigger();

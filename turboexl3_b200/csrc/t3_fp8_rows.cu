@@ -165,14 +165,19 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 for (uint32_t kb = kbs * rank / a.split, i = 0; kb < kbs * (rank + 1u) / a.split && i < a.stages; ++kb, ++i)
                     tma_prefetch_2d(&maps.w[0], (int)(kb * 128u), (int)(cluster * 128u));
         }
-    } else if (warp == kMmaWarp) {
+    }
+    // (Waited for ahead of the first store to another CTA. Ahead of the allocation: no CTA waits, holding tensor memory, for one that waits for some.)
+    if (a.split > 1u) {
+        __syncwarp();
+        cluster_arrive();
+    }
+    if (warp == kMmaWarp) {
         tmem_alloc(&words[1], kCols);
         tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = words[1];
-    if (a.split > 1u) cluster_arrive();  // (waited for ahead of the first store to another CTA)
     // What this kernel reads of the call's earlier launch waits for that one; what was there before the call (`early`: that launch has waited
     // for it ahead of letting this one start) does not. The next kernel may start once this one's tensor memory is allocated, since its
     // CTAs may hold theirs while they wait, and this one's own wait is over.
