@@ -360,3 +360,28 @@ def test_the_exl3_layer_takes_the_same_routing():
     want = sum(scores[..., k:k + 1] * t3.moe(x, exl3, inds[..., k:k + 1].contiguous(), torch.ones_like(scores[..., :1])).float() for k in range(2))
     # the two experts' outputs are rounded to 16 bits once more here than in the layer, and so is their sum
     assert torch.all((y.float() - want).abs() <= 4 * 2.0 ** -11 * (want.abs() + y.float().abs().amax()))
+
+
+@pytest.mark.parametrize("rows,hidden,inter,experts,topk", [(12, 512, 2048, 64, 9), (3, 640, 1792, 46, 8), (32, 1024, 512, 8, 2), (1, 384, 256, 30, 5)])
+def test_calls_behind_one_another_leave_each_other_alone(rows, hidden, inter, experts, topk):
+    """Many calls in a row, each launch starting while the one before it ends: every one gives the first one's bytes."""
+    b, _ = bank(experts, hidden, inter, 71)
+    x = activations(rows, hidden, torch.bfloat16, 4).view(1, rows, hidden)
+    r = t3.route(torch.randn(1, rows, experts, generator=torch.Generator("cuda").manual_seed(1), device="cuda"), topk)
+    w, ws = weights((1100, hidden), 5)
+    first = t3.moe_fp8(x, b, *r), t3.linear_fp8(x, w, ws)
+    got = [(t3.moe_fp8(x, b, *r), t3.linear_fp8(x, w, ws)) for _ in range(200)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(m, first[0]) and torch.equal(l, first[1]) for m, l in got)
+    assert t3.device_error() == 0
+
+
+@pytest.mark.parametrize("rows,width,out", [(1, 2048, 384), (20, 4096, 640), (40, 7168, 130), (200, 7168, 576), (300, 256, 1000)])
+def test_linears_behind_one_another_leave_each_other_alone(rows, width, out):
+    x = activations(rows, width, torch.bfloat16, 6)
+    w, ws = weights((out, width), 7)
+    first = t3.linear_fp8(x, w, ws)
+    got = [t3.linear_fp8(x, w, ws) for _ in range(200)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, first) for y in got)
+    assert t3.device_error() == 0

@@ -118,14 +118,14 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     p.up.cap = p.down.cap = cap;
     p.up.quantise = true, p.down.quantise = false;
     // gate|up. Few tasks: a CTA a multiprocessor, as many slices as that leaves, and room beside it for down's, which start on their weights while
-    // these finish (one row of 512 experts of 2048 x 512: 15.8 -> 13.2 us). Else four slices, two CTAs a multiprocessor. As many slices in
+    // these finish (one row of 512 experts of 2048 x 512: 15.8 -> 13.2 us). Else four slices of at least four blocks, two CTAs a multiprocessor. As many slices in
     // any case as leave the quantised rows' slice room for weights.
     const uint32_t tasks = p.used_max * ik;
     auto too_long = [&](uint32_t t) { return div_up(hk, t) * cap * 128u > 32u * 1024u; };
     uint32_t s = tasks <= resident(1, 1) ? slices_alone(tasks, hk) : 1u;
     const bool pair = tasks > resident(1, 1) || too_long(s);
     if (pair)
-        for (s = 1; s < kFp8SplitMax && s * 2u <= hk && (s < 4u || too_long(s));) s *= 2u;
+        for (s = 1; s < kFp8SplitMax && s * 2u <= hk && ((s < 4u && hk >= 8u * s) || too_long(s));) s *= 2u;
     p.up.split = s, p.up.slice_max = div_up(hk, s);
     if (!fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots, pair, pair ? kOne : kBeside) &&
         !fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots, true))

@@ -148,6 +148,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                 if (i >= ahead && ++rkb == k1) rkb = k0, rt += stride;
             }
             if (a.early && units == 0u) pdl_wait();
+#pragma unroll 1
+            for (uint32_t i = 0; i < kStages; ++i) {  // the last products' arrivals are in before the CTA may end
+                fp8_wait_here<false>(empty + 8u * slot, parity, dead, a.err, kErrEmptyWait);
+                if (++slot == kStages) slot = 0, parity ^= 1u;
+            }
         } else if (warp == kMmaWarp) {
             uint32_t slot = 0, parity = 0, acc = 0, acc_parity = 1;
     #pragma unroll 1
@@ -271,8 +276,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
         __syncwarp();
     }
     if (SPLIT) {
-        cluster_arrive_relaxed();
+        // (a CTA arrives once all that was sent to it is there: past the barrier no copy reads from a CTA any more, nor writes to one)
         fp8_wait_here<true>(recv, 0, dead, a.err, kErrFullWait);
+        __syncwarp();
+        cluster_arrive_relaxed();
         if (a.early) pdl_wait();
         const uint32_t width = N / split, row0 = first % row_tiles * 128u, col0 = first / row_tiles * N + rank * width;
         const float* p = reinterpret_cast<const float*>(smem + (part - base));
@@ -287,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
             store_act(a.y, a.y_dt, (size_t)(row0 + r) * a.out + col0 + n, v);
         }
         __syncwarp();
-        cluster_wait();  // no CTA leaves while another may still write to it
+        cluster_wait();
     }
 }
 

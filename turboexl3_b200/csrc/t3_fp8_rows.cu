@@ -339,6 +339,11 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
             __syncwarp();
             cluster_wait();
         }
+#pragma unroll 1
+        for (uint32_t i = 0; i < a.stages; ++i) {  // the last products' arrivals are in before the CTA may end
+            fp8_wait(bars + kBarEmpty + 8u * s.i, s.parity ^ 1u, dead, a.err, kErrEmptyWait);
+            s.next(a.stages);
+        }
     } else if (warp == kMmaWarp) {
         Slot s, c;
         uint32_t k = 0;  // gate|up, QUANT: the block's place in the slice, each twice
@@ -556,9 +561,14 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
         tmem_dealloc(tmem, kCols);  // ahead of the wait for the other CTAs: they may be waiting for tensor memory themselves
         __syncwarp();
     }
-    if (a.split > 1u) cluster_arrive_relaxed();  // no CTA leaves while another may still write to it
+    // No CTA leaves while another may still write to it, nor while a copy may still read from it: linear's and down's arrive at the cluster's barrier
+    // once all that was sent to them is there, so past it every copy is over.
+    if (MODE != kFp8GateUp && a.split > 1u) {
+        fp8_wait<true>(bars + kBarRecvFull, 0, dead, a.err, kErrFullWait);
+        __syncwarp();
+    }
+    if (a.split > 1u) cluster_arrive_relaxed();
     if (MODE != kFp8GateUp) {
-        if (a.split > 1u) fp8_wait<true>(bars + kBarRecvFull, 0, dead, a.err, kErrFullWait);
         if (early) pdl_wait();
         // a lane four outputs of a column, a warp a column
         const uint32_t own = (CAP + a.split - 1u) / a.split, o = cluster * 128u + 4u * lane;
