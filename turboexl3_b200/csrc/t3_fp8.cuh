@@ -108,6 +108,7 @@ __device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volati
 template <bool CLUSTER = false>
 __device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
     if (!fp8_try<CLUSTER>(bar, parity)) fp8_wait_slow<CLUSTER>(bar, parity, dead, err, bit);
+    __syncwarp();  // (whole warps wait)
 }
 
 // `bytes` (4 or 16) from global to shared memory, in this thread's copy group

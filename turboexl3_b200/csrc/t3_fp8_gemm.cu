@@ -68,6 +68,13 @@ __device__ __forceinline__ uint32_t pack_as(float a, float b, int dt) {
     return *reinterpret_cast<const uint32_t*>(&o);
 }
 
+// a whole warp's wait, in place
+template <bool CLUSTER>
+__device__ __forceinline__ void whole_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+    fp8_wait_here<CLUSTER>(bar, parity, dead, err, bit);
+    __syncwarp();
+}
+
 template <uint32_t N, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                                                          const __grid_constant__ Fp8GemmArgs a) {
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     pdl_trigger();
                 }
                 const uint32_t s = rows_only ? i - ahead : slot, bar = full + 8u * s, at = base + s * kStageBytes;
-                if (!rows_only) fp8_wait_here<false>(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
+                if (!rows_only) whole_wait<false>(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
                 if (elect_one()) {
                     if (!rows_only) {
                         mbar_arrive_expect_tx_addr(bar, kStageBytes);
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
             if (a.early && units == 0u) pdl_wait();
 #pragma unroll 1
             for (uint32_t i = 0; i < kStages; ++i) {  // the last products' arrivals are in before the CTA may end
-                fp8_wait_here<false>(empty + 8u * slot, parity, dead, a.err, kErrEmptyWait);
+                whole_wait<false>(empty + 8u * slot, parity, dead, a.err, kErrEmptyWait);
                 if (++slot == kStages) slot = 0, parity ^= 1u;
             }
         } else if (warp == kMmaWarp) {
@@ -161,8 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                 for (uint32_t kb = k0; kb < k1; ++kb) {
                     const uint32_t at = base + slot * kStageBytes;
                     const uint64_t ad = umma_desc(at), bd = umma_desc(at + kRowBytes);
-                    fp8_wait_here<false>(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
-                    fp8_wait_here<false>(full + 8u * slot, parity, dead, a.err, kErrFullWait);
+                    whole_wait<false>(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
+                    whole_wait<false>(full + 8u * slot, parity, dead, a.err, kErrFullWait);
                     tc_fence_after();
     #pragma unroll
                     for (uint32_t j = 0; j < 4u; ++j)  // 32 inputs each
@@ -202,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     if (kb + p >= k1) break;
                     const float c = sx[p] * sw[p];
                     if (kb + p + 2u < k1) sx[p] = __ldg(xs + kb + p + 2u), sw[p] = __ldg(ws + kb + p + 2u);
-                    fp8_wait_here<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
+                    whole_wait<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
                     tc_fence_after();
                     const uint32_t from = tmem + acc * N + half * kMine + ((quarter * 32u) << 16);
                     // (the next sixteen columns on their way under the multiply-adds of these: 125 -> 115 us at 8192 rows 2048 -> 6144)
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
     }
     if (SPLIT) {
         // (a CTA arrives once all that was sent to it is there: past the barrier no copy reads from a CTA any more, nor writes to one)
-        fp8_wait_here<true>(recv, 0, dead, a.err, kErrFullWait);
+        whole_wait<true>(recv, 0, dead, a.err, kErrFullWait);
         __syncwarp();
         cluster_arrive_relaxed();
         if (a.early) pdl_wait();

@@ -471,8 +471,10 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 // rows, once that has read the last task's.
                 const uint32_t full = bars + kBarRecvFull, mine_of = members & columns, count = __popc(mine_of);
                 if (a.split > 1u) {
-                    if (warp == 0 && lane == 0) mbar_arrive_expect_tx_addr(full, count * a.split * 1024u);
+                    // Only then the arrival of this task's own: a task that sends this CTA nothing ends its phase with it, and a warp that still waited for
+                    // the phase before would find the barrier past two of them, which it cannot tell from none.
                     if (turn) fp8_wait<true>(bars + kBarRecvEmpty, (turn - 1u) & 1u, dead, a.err, kErrEmptyWait);
+                    if (warp == 0 && lane == 0) mbar_arrive_expect_tx_addr(full, count * a.split * 1024u);
                 } else {
                     named_sync(4, kEpiWarps * 32u);  // (both fours have read the last task's)
                 }
