@@ -385,3 +385,43 @@ def test_linears_behind_one_another_leave_each_other_alone(rows, width, out):
     torch.cuda.synchronize()
     assert all(torch.equal(y, first) for y in got)
     assert t3.device_error() == 0
+
+
+def test_a_mix_on_four_streams():
+    """Routed layers and linears of several shapes, EXL3 linears and routings, drawn at random onto four streams: each call gives the bytes it
+    gives alone."""
+    import random
+    jobs = []
+
+    def job(call):
+        alone = call()
+        torch.cuda.synchronize()
+        jobs.append((call, alone))
+
+    for rows, hidden, inter, experts, topk in ((12, 512, 1024, 32, 5), (1, 1024, 512, 64, 8), (29, 1024, 256, 64, 6), (32, 256, 512, 8, 2)):
+        b, _ = bank(experts, hidden, inter, rows)
+        x = activations(rows, hidden, torch.bfloat16, rows).view(1, rows, hidden)
+        r = t3.route(torch.randn(1, rows, experts, device="cuda"), topk)
+        job(lambda x=x, b=b, r=r: t3.moe_fp8(x, b, *r))
+    for rows, width, out in ((1, 2048, 2048), (29, 8192, 512), (200, 7168, 576), (900, 512, 3001), (17, 512, 20000), (64, 4096, 300)):
+        w, ws = weights((out, width), out)
+        x = activations(rows, width, torch.float16, rows)
+        job(lambda x=x, w=w, ws=ws: t3.linear_fp8(x, w, ws))
+    trellis = torch.randint(-32768, 32768, (64, 64, 64), device="cuda", dtype=torch.int16)
+    ones = torch.ones(1024, device="cuda", dtype=torch.float16)
+    for rows in (1, 100):
+        x = torch.randn(rows, 1024, device="cuda").half()
+        job(lambda x=x: t3.linear(x, trellis, ones, ones))
+    logits, bias = torch.randn(500, 256, device="cuda"), 0.1 * torch.randn(256, device="cuda")
+    job(lambda: t3.route(logits, 8, "sigmoid", bias, 8, 4)[0])
+    rng, streams = random.Random(1), [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(15):
+        done = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    call, alone = rng.choice(jobs)
+                    done.append((call(), alone))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, alone) for y, alone in done)
+    assert t3.device_error() == 0

@@ -9,7 +9,6 @@
 
 namespace t3 {
 
-constexpr uint32_t kFp8Group = 128;       // values of a row (and rows of a weight) that share a scale
 constexpr uint32_t kFp8ExpertsMax = 2048; // of a bank: a CTA keeps a word for each
 constexpr uint32_t kFp8SplitMax = 8;      // K slices of a tile: the portable cluster size
 

@@ -131,7 +131,7 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
         !fit(kFp8GateUp, p.up, 2u * p.up.slice_max, (uint32_t)b.experts, slots, true))
         return false;
     const uint32_t most = resident(p.up.per_sm, s) / s;
-    p.clusters = tasks < most ? tasks : most;
+    p.clusters = tasks < most ? tasks : most < 1u ? 1u : most;
     // down: one tile a cluster, as many slices as are resident at once
     s = 1;
     for (uint32_t t = 2; t <= kFp8SplitMax; ++t)  // (with room to spare: they are placed among gate|up's last CTAs, and a cluster that is left over is 20 us)

@@ -6,7 +6,8 @@
 // K-major as it lies in memory) against the same 128 inputs of the rows (B, 16 or 32 of them), so D [128 outputs x rows] lies in
 // tensor memory with an output a lane, and the block's scale and a row's multiply its columns: the epilogue warps add c * D to f32
 // sums in registers, since a scale changes every 128 inputs. Bound by the weight's bytes: a block is 16 KB, 700 cycles of a
-// multiprocessor's share of memory, against 128 cycles of tensor core and some 60 instructions of epilogue.
+// multiprocessor's share of memory, against 128 cycles of tensor core and some 60 instructions of epilogue. 29 rows: 16384 -> 7168 in 26.4 us with the
+// rows' quantising ahead (117 MB), a layer of 512 experts of 2048 x 512 in 125 us (700 MB).
 //
 // K is cut into slices, a CTA of a thread-block cluster each; the slices' sums meet in the cluster's shared memory, each CTA
 // adding the columns n = rank, rank + split, .. in slice order, so the result does not depend on timing.

@@ -5,7 +5,8 @@
 // through each lane's values. Without bias or groups the pick is the logit itself (both scorings rise with it); with them it is score + bias,
 // where two sums that differ in the last bits must still order as their exact values do: they are taken in 32 bits, and those that
 // a choice hangs on and that are too near each other once more in 64. (All rows in 64 bits: 27.5 us at 8192 rows of 256 experts.) Bound by
-// the instructions of the rounds on long prompts, some nine hundred a row, by latency on decode rows.
+// instructions on long prompts (1660 a row of 256 experts in 8 groups, 18.7 us at 8192 rows; 40 % of them the rounds), by latency on decode rows
+// (4.7 us at one row of 512, ten rounds).
 #include "t3_fp8.cuh"
 #include "t3_fp8.h"
 #include "t3_internal.h"
@@ -55,8 +56,7 @@ __device__ __noinline__ double sigmoid_pick(float v, const float* bias, uint32_t
 }
 
 // The picks of one row in 64 bits and the choice among them, for the rows whose order 32 bits leave open and sigmoid_pick of a few experts does
-// not settle: mine [experts] doubles of the
-// warp's. Returns lane k's k-th choice, its highest bit set for a removed expert.
+// not settle: mine [experts] doubles of the warp's. Returns lane k's k-th choice, its highest bit set for a removed expert.
 __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, float top, double* mine, uint32_t lane) {
     double total = 0.0;
 #pragma unroll 1
