@@ -425,3 +425,78 @@ def test_a_mix_on_four_streams():
         torch.cuda.synchronize()
         assert all(torch.equal(y, alone) for y, alone in done)
     assert t3.device_error() == 0
+
+
+# ---- where a tensor starts and how far it reaches ----
+
+def test_scales_and_routing_on_their_own_types_alignment():
+    """Only activations, e4m3 values and outputs have to start on 16 bytes."""
+    def moved(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        room[1:] = t.reshape(-1)
+        return room[1:].view(t.shape)
+    for rows in (3, 31, 70):
+        x = activations(rows, 640, torch.bfloat16, rows)
+        w, ws = weights((200, 640), 2)
+        q, s = t3.quantize_fp8(x)
+        assert torch.equal(t3.linear_fp8(x, w, moved(ws)), t3.linear_fp8(x, w, ws))
+        assert torch.equal(t3.linear_fp8(q, w, moved(ws), moved(s)), t3.linear_fp8(q, w, ws, s))
+    b, _ = bank(6, 256, 384, 3)
+    off = t3.Fp8Bank(*[t3.Fp8Proj(p.w, moved(p.scale)) for p in (b.gate, b.up, b.down)])
+    x = activations(9, 256, torch.float16, 1).view(1, 9, 256)
+    logits = torch.randn(1, 9, 6, device="cuda").bfloat16()
+    bias = torch.rand(6, device="cuda")
+    inds, scores = t3.route(logits, 3, "sigmoid", bias)
+    got = t3.route(moved(logits), 3, "sigmoid", moved(bias))
+    assert torch.equal(got[0], inds) and torch.equal(got[1], scores)
+    assert torch.equal(t3.moe_fp8(x, off, moved(inds), moved(scores.half())), t3.moe_fp8(x, b, inds, scores.half()))
+    assert t3.device_error() == 0
+
+
+def test_quantize_past_32_bits():
+    rows, width = 600000, 7168
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
+    x[-70:] = activations(70, width, torch.bfloat16, 1)
+    q, s = t3.quantize_fp8(x)
+    want_q, want_s = ref.quantize(x[-70:])
+    assert torch.equal(q[-70:].double(), want_q) and torch.equal(s[-70:].double(), want_s)
+    assert float(s[-71].max()) == 2.0 ** -126 and int(q[-71].view(torch.uint8).max()) == 0
+
+
+@pytest.mark.parametrize("rows,width", [(1, 32768), (30, 32768), (40, 32768), (8000, 128)])
+def test_linear_past_32_bits(rows, width):
+    """Weights of more than 4 GiB, and outputs."""
+    out, end = 1094 * 128, 384
+    w = torch.zeros(out, width, dtype=torch.uint8, device="cuda").view(E4M3)
+    ws = torch.ones(out // 128, width // 128, device="cuda")
+    tail, tail_s = weights((end, width), 7)
+    w.view(torch.uint8)[-end:] = tail.view(torch.uint8)
+    ws[-end // 128:] = tail_s
+    x = activations(rows, width, torch.bfloat16, rows)
+    q, s = t3.quantize_fp8(x)
+    y = t3.linear_fp8(q, w, ws, s, torch.float32)
+    part = slice(max(0, rows - 200), rows)
+    want, err = ref.linear(*ref.quantize(x[part]), tail, tail_s)
+    held(y[part, -end:], want, ref.out_bound(want, err, torch.float32))
+    assert int(torch.count_nonzero(y[:, :-end])) == 0
+    assert t3.device_error() == 0
+
+
+def test_moe_past_32_bits():
+    experts, hidden, inter, end = 2048, 2048, 1152, 8
+    small, parts = bank(end, hidden, inter, 5)
+
+    def behind(p):
+        w = torch.zeros((experts,) + p.w.shape[1:], dtype=torch.uint8, device="cuda")
+        s = torch.ones((experts,) + p.scale.shape[1:], device="cuda")
+        w[-end:], s[-end:] = p.w.view(torch.uint8), p.scale
+        return t3.Fp8Proj(w.view(E4M3), s)
+    big = t3.Fp8Bank(*[behind(p) for p in (small.gate, small.up, small.down)])
+    for rows in (1, 4, 20):
+        x = activations(rows, hidden, torch.bfloat16, rows).view(1, rows, hidden)
+        inds = torch.randint(0, end, (1, rows, 2), device="cuda", dtype=torch.int32)
+        scores = torch.rand(1, rows, 2, device="cuda")
+        y = t3.moe_fp8(x, big, inds + (experts - end), scores)[0]
+        want, err = ref.moe(x[0], *parts, inds[0].long(), scores[0])
+        held(y, want, ref.out_bound(want, err, x.dtype))
+    assert t3.device_error() == 0
