@@ -125,3 +125,35 @@ def test_python_refusals():
             call()
     with pytest.raises(RuntimeError, match="contiguous"):
         t3.route(x.t(), 2)
+
+
+def biased_rows(experts, seed, dtype=torch.float32):
+    """Ordinary rows, rows that differ in their last bits, equal ones, and rows with removed experts."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(24, experts, generator=gen) * 2
+    x[6:12] = torch.randint(-2, 3, (6, experts), generator=gen).float()
+    x[9:12] += 2.0 ** -22 * torch.randint(-2, 3, (3, experts), generator=gen)
+    x[12:18] = torch.where(torch.rand(6, experts, generator=gen) < 0.5, -math.inf, x[12:18])
+    x[18:20] = torch.finfo(dtype).min
+    x[20] = 0.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("experts,groups,group_topk,topk", [(8, 1, 1, 4), (4, 1, 1, 4), (64, 1, 1, 6), (160, 1, 1, 32), (8, 4, 2, 3), (16, 8, 3, 5),
+                                                            (6, 3, 2, 4), (64, 8, 4, 8), (256, 8, 4, 8), (32, 32, 7, 7), (1024, 16, 5, 20)])
+def test_a_bias_of_minus_infinity_puts_an_expert_last_and_removes_none(scoring, dtype, experts, groups, group_topk, topk):
+    """Its pick is the lowest number there is; the expert is live: behind every other live one, ahead of a removed one, with its own score, and in its
+    group's sum of two. A few finite biases, one, none; one -inf a group of two."""
+    x = biased_rows(experts, experts + groups, dtype)
+    gen = torch.Generator().manual_seed(groups)
+    some = 0.25 * torch.randint(-1, 2, (experts,), generator=gen).float()
+    for finite in (0, 1, 2, topk - 1, topk, topk + 1, experts - experts // 4, experts):
+        b = torch.full((experts,), -math.inf)
+        keep = torch.randperm(experts, generator=gen)[: min(finite, experts)]
+        b[keep] = some[keep]
+        got_i, got_s = t3.route(x.cuda(), topk, scoring, b.cuda(), groups, group_topk, True, 1.0)
+        want_i, want_s = ref.route(x, topk, scoring, b, groups, group_topk, True, 1.0)
+        assert torch.equal(got_i.cpu().long(), want_i), (finite, (got_i.cpu() != want_i).any(-1).nonzero().view(-1).tolist())
+        close(got_s, want_s)

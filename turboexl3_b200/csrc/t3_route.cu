@@ -7,6 +7,8 @@
 // a choice hangs on and that are too near each other once more in 64. (All rows in 64 bits: 27.5 us at 8192 rows of 256 experts.) Bound by
 // instructions on long prompts (1660 a row of 256 experts in 8 groups, 18.7 us at 8192 rows; 40 % of them the rounds), by latency on decode rows
 // (4.7 us at one row of 512, ten rounds).
+#include <cfloat>
+
 #include "t3_fp8.cuh"
 #include "t3_fp8.h"
 #include "t3_internal.h"
@@ -55,15 +57,20 @@ __device__ __noinline__ double sigmoid_pick(float v, const float* bias, uint32_t
     return bias ? p + (double)bias[e] : p;
 }
 
+// Whether expert e of the row is removed: asked of its logit, since a pick of -inf is a live expert's too, whose bias is.
+__device__ __noinline__ bool removed(const RouteArgs& a, size_t at, uint32_t e) { return load_act(a.logits, a.dt, at + e) <= lowest(a.dt); }
+
 // The picks of one row in 64 bits and the choice among them, for the rows whose order 32 bits leave open and sigmoid_pick of a few experts does
 // not settle: mine [experts] doubles of the warp's. Returns lane k's k-th choice, its highest bit set for a removed expert.
 __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, float top, double* mine, uint32_t lane) {
     double total = 0.0;
+    uint32_t gone = 0;  // a bit for each 32 experts: this lane's is removed
 #pragma unroll 1
     for (uint32_t e = lane; e < a.experts; e += 32u) {
         const float v = load_act(a.logits, a.dt, at + e);
         double p = -INFINITY;
         if (!(v <= lowest(a.dt))) p = a.scoring == 0 ? exp((double)v - (double)top) : sigmoid_pick(v, a.bias, e), total += p;
+        else gone |= 1u << (e >> 5);
         mine[e] = p;
     }
     total = warp_sum(total);
@@ -80,12 +87,14 @@ __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, floa
     if (a.groups > 1u) {
         double first = -INFINITY, second = -INFINITY;
         bool bad = false;
+        uint32_t live = 0;
         const uint32_t lanes = group_lanes(a.groups), g = lane / lanes;
         if (g < a.groups)
 #pragma unroll 1
             for (uint32_t i = lane & (lanes - 1u); i < wide; i += lanes) {
                 const double p = mine[g * wide + i];
                 bad |= isnan(p);
+                live += p != -INFINITY || !removed(a, at, g * wide + i);
                 second = fmax(second, fmin(first, p));
                 first = fmax(first, p);
             }
@@ -93,10 +102,12 @@ __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, floa
         for (uint32_t d = lanes >> 1; d; d >>= 1) {
             const double f = __shfl_xor_sync(kFull, first, d), s = __shfl_xor_sync(kFull, second, d);
             bad |= __shfl_xor_sync(kFull, (int)bad, d) != 0;
+            live += __shfl_xor_sync(kFull, live, d);
             second = fmax(fmax(second, s), fmin(first, f));
             first = fmax(first, f);
         }
-        const uint64_t mine_rank = bad ? ~0ull : key_of(second == -INFINITY ? first : first + second);
+        // (a second of -inf is a live one where there are two, and the sum; a group without a live one is the last)
+        const uint64_t mine_rank = bad ? ~0ull : live == 0u ? 0ull : key_of(live == 1u ? first : second == -INFINITY ? second : first + second);
         const uint64_t rank = __shfl_sync(kFull, mine_rank, lane * lanes & 31u);  // lane g: of group g
         uint32_t ahead = 0;
 #pragma unroll 1
@@ -114,8 +125,7 @@ __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, floa
 #pragma unroll 1
         for (uint32_t e = lane; e < a.experts; e += 32u) {
             if (((taken >> (e >> 5)) & 1u) || !((groups_in >> (a.groups > 1u ? e / wide : 0u)) & 1u)) continue;
-            const double p = mine[e];
-            const uint64_t key = p == -INFINITY ? 1ull : key_of(p);
+            const uint64_t key = (gone >> (e >> 5)) & 1u ? 1ull : key_of(mine[e]);
             if (key > best) best = key, at_best = e;
         }
         const uint64_t most = warp_max(best);
@@ -140,7 +150,6 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
     float v[PER];
     uint32_t out = 0;  // a bit for each removed expert of the lane
     float top = -INFINITY;
-    bool nan = false;
     if (a.dt == kF32) {
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j) v[j] = lane + 32u * j < a.experts ? static_cast<const float*>(a.logits)[at + lane + 32u * j] : -INFINITY;
@@ -155,7 +164,7 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
         if (v[j] <= low) out |= 1u << j;
-        else top = fmaxf(top, v[j]), nan |= isnan(v[j]);
+        else top = fmaxf(top, v[j]);
     }
     static_assert(PER <= 32u, "a bit an expert");
     constexpr uint32_t kAll = PER == 32u ? kFull : (1u << (PER % 32u)) - 1u;
@@ -187,6 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
         float* mine = reinterpret_cast<float*>(picks + (size_t)warp * (a.experts + 32u));
         const uint32_t wide = a.experts / a.groups, magic = ((1u << 20) + wide - 1u) / wide;  // e / wide = e magic >> 20, for e < 1024
         const uint32_t lanes = group_lanes(a.groups);
+        bool odd = false;  // a live pick that is no number, or the lowest there is
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j) {
             const uint32_t e = lane + 32u * j;
@@ -197,15 +207,23 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
             }
             if (a.bias && e < a.experts) p += a.bias[e];
             const bool gone = (out >> j) & 1u;
-            nan |= !gone && isnan(p);
+            odd |= !gone && !(p > -INFINITY);
             key[j] = gone ? 1u : key_of(p);
             if (a.groups > 1u && e < a.experts) mine[e + ((e * magic) >> 20) * lanes] = gone ? -INFINITY : p;
             if (e >= a.experts) key[j] = 0;
         }
-        lost = __any_sync(kFull, nan) != 0 || !any;
+        odd = __any_sync(kFull, odd) != 0;
+        lost = !any;
+        if (odd) {
+            bool nan = false;
+#pragma unroll
+            for (uint32_t j = 0; j < PER; ++j) nan |= key[j] == kFull;
+            lost |= __any_sync(kFull, nan) != 0;
+        }
         if (a.groups > 1u) {
             __syncwarp();
-            // a group's rank is by the sum of its two largest picks that are not removed
+            // a group's rank is by the sum of its two largest picks that are not removed: of those in shared memory the removed ones are -inf, and the
+            // live ones of -inf are looked for only where the row has one
             const uint32_t g = lane / lanes;
             float first = -INFINITY, second = -INFINITY;
             if (g < a.groups) {
@@ -223,7 +241,16 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
                 second = fmaxf(fmaxf(second, s), fminf(first, f));
                 first = fmaxf(first, f);
             }
-            const float both = second == -INFINITY ? first : first + second;
+            bool lowest_live = false;
+            if (odd) {
+                if (g < a.groups)
+#pragma unroll 1
+                    for (uint32_t i = lane & (lanes - 1u); i < wide; i += lanes)
+                        lowest_live |= mine[g * (wide + lanes) + i] == -INFINITY && !removed(a, at, g * wide + i);
+#pragma unroll 1
+                for (uint32_t d = lanes >> 1; d; d >>= 1) lowest_live |= __shfl_xor_sync(kFull, (int)lowest_live, d) != 0;
+            }
+            const float both = second == -INFINITY ? (lowest_live ? second : first) : first + second;
             const uint32_t rank = g < a.groups ? key_of(both) : 0u;
             uint32_t ahead = 0;
 #pragma unroll 4
@@ -235,9 +262,11 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
             if (a.group_topk < a.groups) {
                 const uint32_t least = __reduce_min_sync(kFull, in ? rank : kFull), next = __reduce_max_sync(kFull, in ? 0u : rank);
                 const float l = number_of(least), n = number_of(next);
-                if (!(l - n > 2.0f * slack + 0x1p-20f * (fabsf(l) + fabsf(n)))) {  // (two without a live expert too)
+                // (a finite sum is clear of an infinite one; two of -inf are not: one may have no live expert, or be too large for 32 bits)
+                if (!(l - n > 2.0f * slack + 0x1p-20f * (fminf(fabsf(l), FLT_MAX) + fminf(fabsf(n), FLT_MAX)))) {
                     // the groups' sums in 64 bits, of the two of each that are clear of its third; lane o's of group o
                     double sum64 = -INFINITY;
+                    bool none = true;  // no live expert
                     bool settled = a.scoring != 0;
                     if (lane < a.groups) {
                         float one = -INFINITY, two = -INFINITY, three = -INFINITY;
@@ -251,13 +280,18 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
                             else three = fmaxf(three, q);
                         }
                         settled &= two == -INFINITY || three == -INFINITY || two - three > slack + 0x1p-21f * (fabsf(two) + fabsf(three));
-                        if (settled && one != -INFINITY) {
+                        bool low = false;  // a live pick of -inf
+                        if (odd && two == -INFINITY)
+#pragma unroll 1
+                            for (uint32_t i = 0; i < wide; ++i) low |= p[i] == -INFINITY && !removed(a, at, lane * wide + i);
+                        none = one == -INFINITY && !low;
+                        if (settled && one != -INFINITY && !low) {
                             sum64 = sigmoid_pick(load_act(a.logits, a.dt, at + lane * wide + i1), a.bias, lane * wide + i1);
                             if (two != -INFINITY) sum64 += sigmoid_pick(load_act(a.logits, a.dt, at + lane * wide + i2), a.bias, lane * wide + i2);
                         }
                     }
                     lost |= __any_sync(kFull, !settled) != 0;
-                    const uint64_t mine64 = key_of(sum64);
+                    const uint64_t mine64 = none ? 0ull : key_of(sum64);
                     uint32_t before = 0;
 #pragma unroll 1
                     for (uint32_t o = 0; o < a.groups; ++o) {
@@ -287,6 +321,7 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
     for (uint32_t j = 1; j < PER; ++j) best = max(best, key[j]);
     auto near = [&](uint32_t high, uint32_t low_key) {
         const float l = number_of(high), n = number_of(low_key);
+        if (isinf(l) || isinf(n)) return false;  // a bias is: equal ones are equal in 64 bits too, and the lower number has been taken first
         return !(l - n > slack + 0x1p-21f * (fabsf(l) + fabsf(n)));
     };
 #pragma unroll 1
