@@ -324,8 +324,8 @@ void t3_release_engines(void);
  * with `bias` (f32 [experts], or null) or groups > 1 the largest picks, pick = score + bias in 64 bits (the scores returned are
  * without it). groups > 1: the experts are cut into `groups` equal runs, and only the group_topk runs with the largest sums of
  * their two largest picks are chosen from (the lower run first among equals). renormalise: the chosen scores are divided by their
- * sum (zeros where that is 0); then all are multiplied by `scale`. A logit at or below its type's lowest finite number removes its expert: it
- * counts in no sum, is chosen only where too few others are left, and then has score 0 (a row with nothing left: all scores 0). A bias of
+ * sum, in the ratios that they have before they are rounded to 32 bits (zeros where none of them is live); then all are multiplied by
+ * `scale`. A logit at or below its type's lowest finite number removes its expert: it counts in no sum, is chosen only where too few others are left, and then has score 0 (a row with nothing left: all scores 0). A bias of
  * -inf removes nobody: its expert is behind every other live one and ahead of the removed, counts in its run's sum of two, and has its own score. A NaN
  * logit ranks first and shows in the scores. experts 1..1024, topk 1..32 and no more than can be chosen from, groups 1..32 and a divisor of
  * experts, group_topk 1..groups (1 with one group), scale finite, else BadExl3Shape. */

@@ -157,3 +157,25 @@ def test_a_bias_of_minus_infinity_puts_an_expert_last_and_removes_none(scoring, 
         want_i, want_s = ref.route(x, topk, scoring, b, groups, group_topk, True, 1.0)
         assert torch.equal(got_i.cpu().long(), want_i), (finite, (got_i.cpu() != want_i).any(-1).nonzero().view(-1).tolist())
         close(got_s, want_s)
+
+
+@pytest.mark.parametrize("scoring,bias", [("sigmoid", False), ("sigmoid", True), ("softmax", True)])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_renormalised_scores_of_chosen_experts_far_below_one(scoring, bias, groups):
+    """Scores that 32 bits hold with few bits or not at all still have a ratio: sigmoids of logits far below zero, and softmax's of experts that a
+    bias chose far below the largest logit."""
+    gen = torch.Generator().manual_seed(groups)
+    n = 64
+    x = torch.stack([shift + torch.randn(n, generator=gen) for shift in (-60.0, -80.0, -87.0, -92.0, -100.0, -104.0, -150.0, -600.0)])
+    x[5, ::2] = -math.inf
+    b = torch.zeros(n)
+    if scoring == "softmax":
+        x[:, 3] = 0.0  # takes all of the softmax, and is chosen last
+        b[3] = -9.0
+    if bias:
+        b[10:40:3] += 0.5
+    got_i, got_s = t3.route(x.cuda(), 5, scoring, b.cuda() if bias else None, groups, max(1, groups // 2), True, 2.5)
+    want_i, want_s = ref.route(x, 5, scoring, b if bias else None, groups, max(1, groups // 2), True, 2.5)
+    assert torch.equal(got_i.cpu().long(), want_i)
+    assert torch.all(got_s.sum(-1).cpu() > 2.49)
+    close(got_s, want_s)

@@ -136,6 +136,13 @@ __device__ __noinline__ uint32_t choose_wide(const RouteArgs& a, size_t at, floa
     return chosen;
 }
 
+// A lane's score times a number of the row's own, for scores that 32 bits hold with few bits or as 0: what divides them by their sum needs
+// their ratios alone. The largest's exponential is 1.
+__device__ __noinline__ float in_ratio(float logit, bool counts, int scoring) {
+    const float most = number_of(warp_max(counts ? key_of(logit) : 0u));
+    return counts ? expf(logit - most) / (scoring == 0 ? 1.0f : 1.0f + expf(logit)) : 0.0f;
+}
+
 // PER: experts a lane; WIDE: picks of score + bias
 template <uint32_t PER, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant__ RouteArgs a) {
@@ -393,16 +400,16 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
             chosen &= 0x7FFFFFFFu;
         }
     }
-    float score = 0.0f;
-    if (lane < a.topk && !gone) {
-        const float l = load_act(a.logits, a.dt, at + chosen);
+    float score = 0.0f, l = 0.0f;
+    const bool counts = any && lane < a.topk && !gone;
+    if (counts) {
+        l = load_act(a.logits, a.dt, at + chosen);
         const float e = expf(a.scoring == 0 ? l - top : -fabsf(l));  // the sigmoid by the exponential that cannot overflow
         score = a.scoring == 0 ? e / sum : (l < 0.0f ? e : 1.0f) / (1.0f + e);
     }
-    if (!any) score = 0.0f;
     if (a.renormalise) {
-        float all = score;
-        for (uint32_t d = 16; d; d >>= 1) all += __shfl_xor_sync(kFull, all, d);
+        float all = warp_sum(score);
+        if (all < 0x1p-16f) score = in_ratio(l, counts, a.scoring), all = warp_sum(score);
         score = all == 0.0f ? 0.0f : score / all;
     }
     if (lane < a.topk) {
