@@ -500,3 +500,26 @@ def test_moe_past_32_bits():
         want, err = ref.moe(x[0], *parts, inds[0].long(), scores[0])
         held(y, want, ref.out_bound(want, err, x.dtype))
     assert t3.device_error() == 0
+
+
+@pytest.mark.parametrize("rows,width,out", [(20, 4096, 640), (40, 7168, 130), (200, 7168, 576), (300, 1024, 1000), (1500, 512, 2048)])
+def test_linears_behind_one_another_read_their_own_rows_scales(rows, width, out):
+    """Calls in a row, in a stream and in a graph, on rows that are another power of two times larger each: the quantised values are the same, at the
+    same address of the workspace, and the scales alone differ. Every output is the first one's times that power, exactly."""
+    x = activations(rows, width, torch.bfloat16, 6)
+    w, ws = weights((out, width), 7)
+    powers = [0, 3, -5, 11, -9, 1, 7, -2]
+    xs = [x * 2.0 ** p for p in powers]
+    first = t3.linear_fp8(x, w, ws, out_dtype=torch.float32)
+    for _ in range(20):
+        got = [t3.linear_fp8(v, w, ws, out_dtype=torch.float32) for v in xs]
+        assert all(torch.equal(y, first * 2.0 ** p) for y, p in zip(got, powers))
+    g = torch.cuda.CUDAGraph()
+    moving = x.clone()
+    with torch.cuda.graph(g):
+        y = [t3.linear_fp8(moving, w, ws, out_dtype=torch.float32) for _ in range(3)]
+    for v, p in zip(xs, powers):
+        moving.copy_(v)
+        g.replay()
+        assert all(torch.equal(r, first * 2.0 ** p) for r in y)
+    assert t3.device_error() == 0

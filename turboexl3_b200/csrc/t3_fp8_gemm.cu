@@ -200,17 +200,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
             float2 sums[kMine / 2u];
 #pragma unroll
             for (uint32_t n = 0; n < kMine / 2u; ++n) sums[n] = make_float2(0.0f, 0.0f);
-            // the scales two blocks ahead of their use, in turns
+            // the scales two blocks ahead of their use, in turns (by plain loads: the rows' may be written by the launch before, after this one has
+            // started, and a load through the read-only path is for what no kernel writes while this one is there)
             float sx[2], sw[2];
 #pragma unroll
-            for (uint32_t p = 0; p < 2u; ++p) sx[p] = k0 + p < k1 ? __ldg(xs + k0 + p) : 0.0f, sw[p] = k0 + p < k1 ? __ldg(ws + k0 + p) : 0.0f;
+            for (uint32_t p = 0; p < 2u; ++p) sx[p] = k0 + p < k1 ? xs[k0 + p] : 0.0f, sw[p] = k0 + p < k1 ? ws[k0 + p] : 0.0f;
 #pragma unroll 1
             for (uint32_t kb = k0; kb < k1; kb += 2u) {
 #pragma unroll
                 for (uint32_t p = 0; p < 2u; ++p) {
                     if (kb + p >= k1) break;
                     const float c = sx[p] * sw[p];
-                    if (kb + p + 2u < k1) sx[p] = __ldg(xs + kb + p + 2u), sw[p] = __ldg(ws + kb + p + 2u);
+                    if (kb + p + 2u < k1) sx[p] = xs[kb + p + 2u], sw[p] = ws[kb + p + 2u];
                     whole_wait<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
                     tc_fence_after();
                     const uint32_t from = tmem + acc * N + half * kMine + ((quarter * 32u) << 16);

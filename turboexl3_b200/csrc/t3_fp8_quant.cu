@@ -18,7 +18,7 @@ constexpr uint32_t kUnder = 4;  // groups a half warp has under way
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) fp8_quantize(const void* __restrict__ x, size_t groups, uint8_t* __restrict__ q, float* __restrict__ scale) {
+__global__ void __launch_bounds__(kThreads) fp8_quantize(const void* x, size_t groups, uint8_t* q, float* scale) {
     constexpr uint32_t kWords = DT == kF32 ? 8u : 4u;
     pdl_wait();
     pdl_trigger();
