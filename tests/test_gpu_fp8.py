@@ -523,3 +523,61 @@ def test_linears_behind_one_another_read_their_own_rows_scales(rows, width, out)
         g.replay()
         assert all(torch.equal(r, first * 2.0 ** p) for r in y)
     assert t3.device_error() == 0
+
+
+@pytest.mark.parametrize("rows,topk", [(1, 4), (5, 3), (32, 8)])
+def test_routings_behind_one_another_at_the_same_addresses(rows, topk):
+    """Routings of changing logits, each ahead of both kinds of routed layer, which read the choice ahead of their second launch's own wait: a captured
+    chain of three, replayed on new logits, whose outputs lie at the same addresses every time, gives the eager calls' bytes."""
+    hidden, inter, experts = 256, 128, 48
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+
+    def proj(i, o):
+        return t3.Proj(torch.randint(-32768, 32768, (experts, i // 16, o // 16, 64), generator=gen, device="cuda", dtype=torch.int16),
+                       torch.full((experts, i), 2.0 ** -4, device="cuda", dtype=torch.float16), torch.ones(experts, o, device="cuda", dtype=torch.float16))
+
+    exl3 = t3.Bank(proj(hidden, inter), proj(hidden, inter), proj(inter, hidden))
+    fp8, _ = bank(experts, hidden, inter, 51)
+    x = activations(rows, hidden, torch.float16, 3).view(1, rows, hidden)
+    logits = [torch.empty(1, rows, experts, device="cuda") for _ in range(3)]
+
+    def chain():
+        out = []
+        for l in logits:
+            inds, scores = t3.route(l, topk)
+            out += [inds, scores, t3.moe(x, exl3, inds, scores), t3.moe_fp8(x, fp8, inds, scores)]
+        return out
+
+    def alone():
+        out = []
+        for l in logits:
+            inds, scores = t3.route(l, topk)
+            torch.cuda.synchronize()
+            for layer, b in ((t3.moe, exl3), (t3.moe_fp8, fp8)):
+                out.append(layer(x, b, inds, scores))
+                torch.cuda.synchronize()
+        return out
+
+    for l in logits:
+        l.normal_(generator=gen)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = chain()
+    before = None
+    for _ in range(12):
+        for l in logits:
+            l.normal_(generator=gen)
+        g.replay()
+        g.replay()
+        eager = chain()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+        assert all(torch.equal(a, b) for a, b in zip([v for i, v in enumerate(got) if i % 4 > 1], alone()))
+        assert before is None or not torch.equal(before, got[0])  # (the choice did change)
+        before = got[0].clone()
+    assert t3.device_error() == 0

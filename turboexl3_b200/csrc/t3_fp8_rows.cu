@@ -188,8 +188,8 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
         pdl_trigger();
     }
 
-    // The routing, on its way while the rows are quantised. It is read past L1: in down the kernel before this one still runs, and what that one
-    // has waited for need not be known to this multiprocessor's cache.
+    // The routing, on its way while the rows are quantised. (In down too it was complete before this launch started, since gate|up lets it start only
+    // after its own wait. A CTA reads each word once, so past L1, where nothing would be found.)
     uint32_t id[kIds];
     if (MODE != kFp8Linear) {
         const uint32_t slots = a.rows * a.topk;
