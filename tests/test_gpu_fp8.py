@@ -581,3 +581,20 @@ def test_routings_behind_one_another_at_the_same_addresses(rows, topk):
         assert before is None or not torch.equal(before, got[0])  # (the choice did change)
         before = got[0].clone()
     assert t3.device_error() == 0
+
+
+@pytest.mark.parametrize("scores_dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,topk", [(3, 2), (16, 2), (32, 5)])
+def test_moe_scores_in_16_bits_are_their_f32_values(scores_dtype, rows, topk):
+    """Few slots and more than a warp's, against 64 bits and, to the byte, against the same scores held in f32."""
+    x = activations(rows, 384, torch.bfloat16, 8)
+    b, parts = bank(7, 384, 128, 5)
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    inds = torch.randint(0, 7, (rows, topk), generator=gen, device="cuda", dtype=torch.int32)
+    scores = (torch.rand(rows, topk, generator=gen, device="cuda") + 0.05).to(scores_dtype)
+    y = check_moe(x, b, parts, inds, scores)
+    assert torch.equal(y, t3.moe_fp8(x[None], b, inds[None], scores.float()[None])[0])
+    # every row to one expert, its slots' scores added up
+    one = torch.full((rows, topk), 2, dtype=torch.int32, device="cuda")
+    y = check_moe(x, b, parts, one, scores)
+    assert torch.equal(y, t3.moe_fp8(x[None], b, one[None].view(torch.uint32), scores.float()[None])[0])
