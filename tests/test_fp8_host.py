@@ -142,3 +142,32 @@ def test_every_layer_has_a_plan(hidden, inter):
                 if experts * max(hidden, inter) < 1 << 31:
                     b = _bank(experts, hidden, inter)
                     assert L.t3_moe_fp8_workspace_bytes(rows, topk, C.byref(b)) > 0
+
+
+class _GemmPlan(C.Structure):
+    _fields_ = [("n", C.c_uint32), ("split", C.c_uint32), ("grid", C.c_uint32)]
+
+
+def _gemm_plan():
+    plan = t3.lib()._ZN2t313plan_fp8_gemmEjjj  # t3::plan_fp8_gemm(rows, in, out)
+    plan.restype, plan.argtypes = _GemmPlan, [C.c_uint32] * 3
+    return plan
+
+
+def test_the_shapes_tested_on_the_device_reach_every_kernel_of_the_gemm():
+    from fp8_shapes import GEMM
+    if torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the plans of 148 multiprocessors")
+    plan = _gemm_plan()
+    for shape, kernel in GEMM.items():
+        p = plan(*shape)
+        assert (p.n, p.split) == kernel, shape
+    reached = set()
+    for rows in list(range(33, 700, 13)) + [1000, 2000, 8192]:
+        for width in list(range(128, 2048, 128)) + list(range(2048, 20481, 512)):
+            for out in (64, 77, 200, 576, 700, 1100, 1601, 3001, 6144):
+                p = plan(rows, width, out)
+                assert p.n in (64, 128, 256) and 1 <= p.grid <= 148 and p.split <= 8 and p.grid % p.split == 0
+                assert p.split == 1 or p.grid == -(-rows // 128) * -(-out // p.n) * p.split
+                reached.add((p.n, p.split))
+    assert reached == set(GEMM.values())

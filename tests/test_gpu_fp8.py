@@ -7,6 +7,7 @@ import torch
 
 import fp8_ref as ref
 import turboexl3_b200 as t3
+from fp8_shapes import GEMM
 
 pytestmark = pytest.mark.gpu
 E4M3 = torch.float8_e4m3fn
@@ -598,3 +599,24 @@ def test_moe_scores_in_16_bits_are_their_f32_values(scores_dtype, rows, topk):
     one = torch.full((rows, topk), 2, dtype=torch.int32, device="cuda")
     y = check_moe(x, b, parts, one, scores)
     assert torch.equal(y, t3.moe_fp8(x[None], b, one[None].view(torch.uint32), scores.float()[None])[0])
+
+
+@pytest.mark.parametrize("rows,width,out", sorted(GEMM))
+def test_every_kernel_of_the_gemm(rows, width, out):
+    """Against 64 bits, the three output types in turn; then calls behind one another, on two streams, give the first one's bytes."""
+    dtype = (torch.bfloat16, torch.float16, torch.float32)[(rows + out) % 3]
+    x = activations(rows, width, dtype, rows)
+    w, ws = weights((out, width), out)
+    y = t3.linear_fp8(x, w, ws)
+    q, s = ref.quantize(x)
+    want, err = ref.linear(q, s, w, ws)
+    held(y, want, ref.out_bound(want, err, dtype))
+    mine, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    side.wait_stream(mine)
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(side if i % 3 == 2 else mine):
+            got.append(t3.linear_fp8(x, w, ws))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, y) for v in got)
+    assert t3.device_error() == 0
