@@ -341,6 +341,7 @@ int t3_quantize_fp8(const void* x, int x_dtype, size_t rows, int in_dim, void* q
 
 /* y [rows, out] in y_dtype = x W^T with W e4m3 [out, in], w_scale f32 [ceil(out / 128), in / 128]: in a multiple of 128, out any. x
  * f32, f16 or bf16 is quantised as t3_quantize_fp8 does it (x_scale null); x_dtype T3_E4M3: x is q, x_scale its scales (any f32 values).
+ * rows times the larger of in and out is below 2^31, and rows at most 4194240, else BadExl3Shape.
  * Products and sums in f32, one rounding into y. The workspace (256-byte aligned) holds the quantised rows where the kernel does not
  * quantise them itself: t3_linear_fp8_workspace_bytes, 0 for T3_E4M3. */
 size_t t3_linear_fp8_workspace_bytes(size_t rows, int in_dim, int out_dim, int x_dtype);
@@ -353,7 +354,9 @@ int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, 
  * 128, experts 1..T3_FP8_EXPERTS_MAX. inds i32 / u32 and scores (scores_dtype) [rows, topk], topk 1..32; an id outside the bank is nobody's and
  * adds nothing, whatever its score (a padded row's, or another rank's of an expert-parallel layer); an id may come twice. shared:
  * [rows, hidden] in x's dtype (on 16 bytes, like y) added before the one rounding, or null. y in x's dtype. Rows 1..T3_DECODE_ROWS_MAX, more:
- * Exl3EngineNotImplemented. Workspace (256-byte aligned): t3_moe_fp8_workspace_bytes. */
+ * Exl3EngineNotImplemented. Every hidden size up to 32768 is served; a larger one as long as a slice of the quantised rows leaves room for
+ * weights in shared memory (up to 79872 at 16 rows or fewer and 34816 past them, whatever the experts and topk), else Exl3EngineNotImplemented and a
+ * workspace of 0. Workspace (256-byte aligned): t3_moe_fp8_workspace_bytes. */
 #define T3_FP8_EXPERTS_MAX 2048
 typedef struct {
     const void* w;

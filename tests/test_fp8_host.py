@@ -171,3 +171,24 @@ def test_the_shapes_tested_on_the_device_reach_every_kernel_of_the_gemm():
                 assert p.split == 1 or p.grid == -(-rows // 128) * -(-out // p.n) * p.split
                 reached.add((p.n, p.split))
     assert reached == set(GEMM.values())
+
+
+@pytest.mark.parametrize("rows,topk,served", [(1, 1, 79872), (16, 32, 79872), (17, 1, 34816), (32, 32, 34816)])
+def test_hidden_sizes_of_the_routed_layer_that_are_served(rows, topk, served):
+    """Every one up to what the header states; past some larger one none, by the same status from the call, and a workspace of 0."""
+    L = t3.lib()
+
+    def need(experts, hidden):
+        return L.t3_moe_fp8_workspace_bytes(rows, topk, C.byref(_bank(experts, hidden, 128)))
+    for experts in (1, 64, 2048):
+        assert all(need(experts, h) > 0 for h in range(128, served + 1, 128))
+        end = next(h for h in range(served, 200000, 128) if need(experts, h) == 0)
+        assert all(need(experts, h) == 0 for h in range(end, end + 40000, 128))
+        for h, status in ((end - 128, "WorkspaceTooSmall"), (end, "Exl3EngineNotImplemented")):
+            assert _moe(bank=_bank(experts, h, 128), rows=rows, topk=topk, work_bytes=16) == status
+
+
+def test_linear_rows_that_are_served():
+    assert _linear(rows=65535 * 64, width=128, out=511, work_bytes=16) == "WorkspaceTooSmall"
+    assert _linear(rows=65535 * 64, width=128, out=513, work_bytes=16) == "BadExl3Shape"
+    assert _linear(rows=65535 * 64 + 1, width=128, out=1, work_bytes=16) == "BadExl3Shape"
