@@ -279,7 +279,7 @@ int t3_linear_unrot(const void* x, int x_dtype, size_t rows, const void* w_std_t
  * current configuration: each kernel takes ONE argument block (DenseArgs / MoeArgs of csrc/t3_internal.h) whose buffers are
  * listed by role, numbered as plan.Role is. They return the number of launches written, or minus a t3_status. Prefill
  * rows (> T3_DECODE_ROWS_MAX): -Exl3EngineNotImplemented. t3_last_kernel_symbol names the kernel the calling thread's last
- * decode-row launch ran (so a test can hold the plan against the launches). */
+ * decode-row launch of an EXL3 call ran (so a test can hold the plan against the launches); the 8-bit layers and the router do not change it. */
 typedef enum {
     T3_ROLE_X, T3_ROLE_SUH, T3_ROLE_SVH, T3_ROLE_TRELLIS, T3_ROLE_XP, T3_ROLE_XS, T3_ROLE_Z, T3_ROLE_Y,
     T3_ROLE_SLOTS, T3_ROLE_SCORES, T3_ROLE_GATE_T, T3_ROLE_UP_T, T3_ROLE_DOWN_T, T3_ROLE_GATE_SUH, T3_ROLE_UP_SUH,
@@ -303,7 +303,8 @@ const char* t3_last_kernel_symbol(void);
 
 /* root.enginesHeld / root.releaseEngines (src/root.zig:1148-1192). The reference caches a compiled engine per geometry and
  * frees them on request; here kernels are compiled ahead and a plan is recomputed per call, so an "engine" is only the
- * record that a geometry was served on a path. The counts are distinct geometries since the last release. */
+ * record that a geometry was served on a path. The counts are distinct geometries since the last release, of the EXL3 calls (the 8-bit
+ * layers' and the router's are in none). */
 typedef struct t3_engines {
     size_t decode;  /* routed GEMV chains (rows <= 32) */
     size_t dense;   /* dense linears at decode rows */

@@ -620,3 +620,22 @@ def test_every_kernel_of_the_gemm(rows, width, out):
     torch.cuda.synchronize()
     assert all(torch.equal(v, y) for v in got)
     assert t3.device_error() == 0
+
+
+def test_the_exl3_records_are_the_exl3_calls_alone():
+    """engines_held counts the geometries of EXL3 calls, as the reference's does; last_kernel_symbol names an EXL3 decode-row kernel."""
+    trellis = torch.randint(-32768, 32768, (16, 16, 64), device="cuda", dtype=torch.int16)
+    ones = torch.ones(256, device="cuda", dtype=torch.float16)
+    t3.release_engines()
+    t3.linear(torch.randn(1, 256, device="cuda").half(), trellis, ones, ones)
+    held_before, symbol = t3.engines_held(), t3.last_kernel_symbol()
+    assert held_before == {"decode": 0, "dense": 1, "prefill": 0}
+    b, _ = bank(4, 256, 128, 3)
+    w, ws = weights((256, 256), 1)
+    for rows in (2, 100):
+        t3.linear_fp8(activations(rows, 256, torch.bfloat16, 1), w, ws)
+    x = activations(3, 256, torch.bfloat16, 1).view(1, 3, 256)
+    t3.moe_fp8(x, b, *t3.route(torch.randn(1, 3, 4, device="cuda"), 2))
+    t3.quantize_fp8(x)
+    assert t3.engines_held() == held_before and t3.last_kernel_symbol() == symbol
+    t3.release_engines()

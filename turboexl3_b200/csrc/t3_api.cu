@@ -182,7 +182,6 @@ uint32_t* device_error_word() { return dev_error_ptr(); }
 bool launches_overlap() { return !config().no_overlap; }
 bool prefill_served() { return config().prefill != 0; }
 void count_launches(int n) { g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed); }
-void note_geometry(int kind, uint64_t a, uint64_t b, uint64_t c, uint64_t d) { note_engine(kind, a, b, c, d); }
 uint32_t multiprocessors() { return one_wave() / 2u; }
 
 uint32_t row_cap_for(uint32_t rows) { return rows <= 8u ? 8u : (rows <= 16u ? 16u : 32u); }

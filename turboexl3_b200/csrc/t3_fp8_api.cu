@@ -213,7 +213,6 @@ int t3_linear_fp8(const void* x, int x_dtype, const void* x_scale, size_t rows, 
     if (!make_byte_map(&maps.w[0], w, out, in, few ? 128u : g.n)) return T3_KERNEL_CREATE_FAILED;
     if (!p.quantise && !make_byte_map(&maps.rows, given ? x : workspace, rows, in, few ? p.cap : 128u)) return T3_KERNEL_CREATE_FAILED;
     const bool overlap = launches_overlap();
-    note_geometry(few ? 1 : 2, in, out, 0, 8);
     if (ahead) {
         count_launches(1);
         if (cudaError_t rc = launch_fp8_quantize(x, x_dtype, rows, in, static_cast<uint8_t*>(workspace), scale, overlap, stream)) return status_of(rc);
@@ -269,7 +268,6 @@ int t3_moe_fp8(const void* x, int x_dtype, size_t rows, const t3_fp8_bank* bank,
     a.h = static_cast<uint8_t*>(workspace), a.h_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.h_scale);
     a.err = device_error_word();
     const bool overlap = launches_overlap();
-    note_geometry(0, hidden, inter, experts, 8);
     count_launches(1);
     if (cudaError_t rc = launch_fp8_rows(kFp8GateUp, cap, up, a, p.clusters, overlap, static_cast<cudaStream_t>(stream)))
         return status_of(rc);

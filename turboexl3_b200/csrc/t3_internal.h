@@ -123,12 +123,11 @@ cudaError_t launch_overlapped(void (*fn)(Params...), dim3 grid, uint32_t block, 
 }
 
 // What the entry points of every translation unit share with t3_api.cu: the current device's error word (null without a device),
-// whether launches may overlap their predecessor, the launch count, the geometries served (kind 0 decode chains, 1 dense, 2 prefill)
+// whether launches may overlap their predecessor, the launch count
 uint32_t* device_error_word();
 bool launches_overlap();
 bool prefill_served();  // t3_config.prefill
 void count_launches(int n);
-void note_geometry(int kind, uint64_t a, uint64_t b, uint64_t c, uint64_t d);
 uint32_t multiprocessors();  // of the current device
 // a tensor map of bytes [rows, bytes], boxes of 128 bytes x box_rows, 128-byte swizzle, rows past the end read as zero
 bool make_byte_map(void* map, const void* base, uint64_t rows, uint64_t bytes, uint32_t box_rows);
