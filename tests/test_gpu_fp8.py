@@ -639,3 +639,16 @@ def test_the_exl3_records_are_the_exl3_calls_alone():
     t3.quantize_fp8(x)
     assert t3.engines_held() == held_before and t3.last_kernel_symbol() == symbol
     t3.release_engines()
+
+
+@pytest.mark.parametrize("rows,hidden,inter,experts,topk", [(1, 4096, 2048, 8, 4), (1, 4096, 256, 128, 4), (2, 1024, 256, 2048, 2), (32, 512, 128, 128, 32)])
+def test_moe_whose_down_takes_what_gate_and_up_leave(rows, hidden, inter, experts, topk):
+    """Shapes whose second launch has its weights in flight cut to the shared memory that the first one's CTAs leave a multiprocessor."""
+    x = activations(rows, hidden, torch.bfloat16, rows)
+    b, parts = bank(experts, hidden, inter, 11)
+    scores, inds = torch.randn(rows, experts, generator=torch.Generator().manual_seed(rows)).softmax(-1).cuda().topk(topk)  # (2048: more than route takes)
+    inds = inds.to(torch.int32)
+    y = check_moe(x, b, parts, inds, scores)
+    got = [t3.moe_fp8(x[None], b, inds[None], scores[None])[0] for _ in range(50)]
+    assert all(torch.equal(v, y) for v in got)
+    assert t3.device_error() == 0

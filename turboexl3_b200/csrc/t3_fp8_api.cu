@@ -1,5 +1,6 @@
 // The C entry points of the 8-bit layers and the router (include/t3.h): admission and launch planning. Every refusal comes before
 // any launch.
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
@@ -18,8 +19,9 @@ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
 // Shared memory a CTA may take: where two fit a multiprocessor (228 KB, 1 KB a CTA reserved), and one
 constexpr uint32_t kTwo = 113u * 1024u, kOne = 227u * 1024u;
-constexpr uint32_t kHalfMore = 115u * 1024u;  // no second CTA that takes as much fits beside it; one of up to 106 KB does beside kBeside
+constexpr uint32_t kHalfMore = 115u * 1024u;  // no second CTA that takes as much fits beside it; one of up to 104 KB does beside kBeside
 constexpr uint32_t kBeside = 122u * 1024u;
+constexpr uint32_t beside(uint32_t total) { return 228u * 1024u - 2048u - total; }  // what a CTA may take beside one of `total`
 constexpr uint32_t kStagesMost = 12;
 
 struct RowsPlan {
@@ -44,13 +46,14 @@ uint32_t slices_alone(uint32_t tiles, uint32_t most) {
 
 // Weight tiles in flight: what fits beside the rest. pair: two CTAs a multiprocessor where that leaves each three tiles (a stream of 16 KB tiles, 224
 // CTAs: 5.0 TB/s with two in flight, 5.6 with three or more). Else up to `room` bytes, and at least what keeps a second one of its kind from the
-// multiprocessor: the hardware doubles up CTAs while other multiprocessors are empty, and the late ones set the launch's duration.
-bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots, bool pair, uint32_t room = kOne) {
+// multiprocessor: the hardware doubles up CTAs while other multiprocessors are empty, and the late ones set the launch's duration. two: what a
+// CTA of a pair may take.
+bool fit(int mode, RowsPlan& p, uint32_t units, uint32_t experts, uint32_t slots, bool pair, uint32_t room = kOne, uint32_t two = kTwo) {
     for (uint32_t per = pair ? 2u : 1u; per >= 1u; --per) {
         for (uint32_t stages = kStagesMost < units ? kStagesMost : units < 2u ? 2u : units; stages >= 2u; --stages) {
             if (per == 2u && stages < 3u && stages < units) break;
             const Fp8RowsLayout l = fp8_rows_layout(mode, p.cap, p.quantise, p.slice_max, p.split, stages, experts, slots);
-            if (l.total > (per == 2u ? kTwo : room)) continue;
+            if (l.total > (per == 2u ? two : room)) continue;
             p.stages = stages, p.per_sm = per, p.layout = l;
             if (!pair && p.layout.total < kHalfMore) p.layout.total = kHalfMore;
             return true;
@@ -137,7 +140,10 @@ bool plan_moe(size_t rows, int topk, const t3_fp8_bank& b, MoePlan& p) {
     for (uint32_t t = 2; t <= kFp8SplitMax; ++t)  // (with room to spare: they are placed among gate|up's last CTAs, and a cluster that is left over is 20 us)
         if (hk * t <= resident(2, t) * 7u / 8u) s = t;
     p.down.split = s, p.down.slice_max = 0;
-    if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots, true)) return false;
+    // Where gate|up leaves room, what it leaves: weights in flight past it would keep down's CTAs waiting for its own to end (one row, four of 8
+    // experts of 4096 x 2048, 32 bytes too many: 26.5 -> 26.3 us).
+    const bool room = p.up.per_sm == 1u && p.up.layout.total <= kBeside;
+    if (!fit(kFp8Down, p.down, kStagesMost, (uint32_t)b.experts, slots, true, kOne, room ? std::min(kTwo, beside(p.up.layout.total)) : kTwo)) return false;
     const size_t h = up256((size_t)p.used_max * cap * (size_t)b.inter);
     p.h_scale = h;
     p.total = h + up256((size_t)p.used_max * cap * ik * 4u);
