@@ -14,9 +14,6 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kUnder = 4;  // groups a half warp has under way
 
-// the larger of each half of two words, as whole numbers of 16 bits
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
-
 template <int DT>
 __global__ void __launch_bounds__(kThreads) fp8_quantize(const void* x, size_t groups, uint8_t* q, float* scale) {
     constexpr uint32_t kWords = DT == kF32 ? 8u : 4u;
@@ -45,11 +42,11 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize(const void* x, size_t g
             uint32_t most = 0;
 #pragma unroll
             for (uint32_t k = 0; k < kWords; ++k)
-                most = DT == kF32 ? max(most, w[j][k] & 0x7FFFFFFFu) : max_u16x2(most, w[j][k] & 0x7FFF7FFFu);
+                most = DT == kF32 ? max(most, w[j][k] & 0x7FFFFFFFu) : __vmaxu2(most, w[j][k] & 0x7FFF7FFFu);
 #pragma unroll
             for (uint32_t d = 8; d; d >>= 1) {
                 const uint32_t other = __shfl_xor_sync(half, most, d);
-                most = DT == kF32 ? max(most, other) : max_u16x2(most, other);
+                most = DT == kF32 ? max(most, other) : __vmaxu2(most, other);
             }
             if (DT == kBf16) most = max(most << 16, most & 0xFFFF0000u);
             if (DT == kF16) most = __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(most & 0xFFFFu, most >> 16))));

@@ -25,8 +25,6 @@
 // of up (the second's); its CTAs quantise silu(gate) * up and leave it as e4m3 for the rows that chose the expert. Down's tile is 128
 // outputs over all experts in use (K runs over expert and input), the router's weight in c, so the sum over a row's experts is
 // taken in registers in ascending order of the experts' numbers: no atomics, no third launch.
-#include <type_traits>
-
 #include "t3_fp8.cuh"
 #include "t3_fp8.h"
 #include "t3_internal.h"
