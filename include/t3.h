@@ -112,6 +112,9 @@ int t3_device_error(void* stream, uint32_t* bits_out, int clear);
  * about a second the wait gives up, bit 0 (a copy never landed) is set in the error word and the kernel returns: what a
  * stalled copy looks like to the host. Nothing faults and the context stays usable. */
 int t3_selftest_wait_runs_out(void* stream);
+/* The same for the 8-bit kernels' waits, one behind the other: a second and a half until the first gives up, bit 2 (a tensor-core completion never
+ * arrived) is set, and the second, for another phase nothing completes, gives up at once. */
+int t3_selftest_fp8_wait_runs_out(void* stream);
 
 /* W_hat: the inner f16 weight [in, out] (format.reconstructInner, src/core/format.zig:276-291;
  * Dense.dequantize, src/core/dense.zig:909-922). */

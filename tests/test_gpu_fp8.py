@@ -652,3 +652,19 @@ def test_moe_whose_down_takes_what_gate_and_up_leave(rows, hidden, inter, expert
     got = [t3.moe_fp8(x[None], b, inds[None], scores[None])[0] for _ in range(50)]
     assert all(torch.equal(v, y) for v in got)
     assert t3.device_error() == 0
+
+
+def test_a_wait_that_runs_out_is_reported_once_and_the_next_calls_run():
+    assert t3.device_error() == 0
+    w, ws = weights((256, 512), 1)
+    x = activations(40, 512, torch.bfloat16, 1)
+    want = t3.linear_fp8(x, w, ws), t3.linear_fp8(x[:3], w, ws)
+    torch.cuda.synchronize()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    assert t3.lib().t3_selftest_fp8_wait_runs_out(torch.cuda.current_stream().cuda_stream) == 0
+    end.record()
+    assert t3.device_error() == 4  # the first wait's bit alone: the second sees that the CTA has given up
+    assert 0.5e3 < start.elapsed_time(end) < 10e3  # milliseconds: bounded, and not by a wait each
+    assert t3.device_error() == 0
+    assert torch.equal(t3.linear_fp8(x, w, ws), want[0]) and torch.equal(t3.linear_fp8(x[:3], w, ws), want[1])

@@ -83,6 +83,7 @@ SYMBOLS = {
     "t3_configure": (_i, [C.POINTER(_Config)]),
     "t3_device_error": (_i, [_vp, C.POINTER(_u32), _i]),
     "t3_selftest_wait_runs_out": (_i, [_vp]),
+    "t3_selftest_fp8_wait_runs_out": (_i, [_vp]),
     "t3_dequant": (_i, [_vp, _i, _i, _i, _Decode, _vp, _vp]),
     "t3_codebook_table": (_i, [_Decode, _vp, _vp]),
     "t3_linear_workspace_bytes": (_sz, [_sz, _i, _i, _i]),

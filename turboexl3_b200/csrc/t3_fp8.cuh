@@ -75,7 +75,10 @@ __device__ __forceinline__ float load_act_cg(const void* p, int dt, size_t i) {
 // before their arrivals is visible after it. The loop is a call: these kernels' code comes from memory again for every launch, behind the
 // weights that have passed through L2, and what it does not hold it does not wait for. (fp8_wait_here: the loop in place, for a caller
 // with so many registers in use that keeping them ready for a call costs more.)
-constexpr uint32_t kFp8Tries = 1u << 22;
+// LAST: the wait that has run out takes some 50 us more, in which what the warp has issued (copies into this CTA's shared memory or out of it,
+// products into its tensor memory) ends. A warp that issues has one behind its last issue, so nothing is under way when the CTA gives its memory
+// back. (A look at `dead` at the CTA's end, or ahead of every issue, cost each call 0.2 to 0.4 us.)
+constexpr uint32_t kFp8Tries = 1u << 20;  // of 1.5 us each
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
@@ -91,19 +94,25 @@ __device__ __forceinline__ bool fp8_try(uint32_t bar, uint32_t parity) {
         done = mbar_try(bar, parity);
     return done != 0u;
 }
-template <bool CLUSTER>
+template <bool CLUSTER, bool LAST>
 __device__ __forceinline__ void fp8_wait_here(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+    uint32_t i = 0;
 #pragma unroll 1
-    for (uint32_t i = 0; i < kFp8Tries; ++i) {
+    for (; i < kFp8Tries; ++i) {
         if (fp8_try<CLUSTER>(bar, parity)) return;
-        if (*dead) return;
+        if (*dead) break;
     }
-    *dead = 1u;
-    if (err) atomicOr(err, bit);
+    if (i == kFp8Tries) {
+        *dead = 1u;
+        if (err) atomicOr(err, bit);
+    }
+    if (LAST)
+#pragma unroll 1
+        for (i = 0; i < 50u; ++i) __nanosleep(1000);
 }
 template <bool CLUSTER>
 __device__ __noinline__ void fp8_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
-    fp8_wait_here<CLUSTER>(bar, parity, dead, err, bit);
+    fp8_wait_here<CLUSTER, true>(bar, parity, dead, err, bit);
 }
 template <bool CLUSTER = false>
 __device__ __forceinline__ void fp8_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {

@@ -73,6 +73,9 @@ cudaError_t launch_fp8_gemm(const CUtensorMap& w, const CUtensorMap& x, const Fp
 // x [rows, in] -> e4m3 values and scales [rows, in / 128]
 cudaError_t launch_fp8_quantize(const void* x, int dt, size_t rows, uint32_t in, uint8_t* q, float* scale, bool overlap, cudaStream_t stream);
 
+// one warp whose waits nothing ends (test hook)
+cudaError_t launch_fp8_wait_runs_out(uint32_t* err, cudaStream_t stream);
+
 struct RouteArgs {
     const void* logits;  // [rows, experts]
     int dt, scoring;

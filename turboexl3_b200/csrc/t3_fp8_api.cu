@@ -162,6 +162,13 @@ using namespace t3;
 
 extern "C" {
 
+int t3_selftest_fp8_wait_runs_out(void* stream) {
+    uint32_t* err = device_error_word();
+    if (!err) return T3_CUDA_ERROR;
+    count_launches(1);
+    return status_of(launch_fp8_wait_runs_out(err, static_cast<cudaStream_t>(stream)));
+}
+
 int t3_route(const void* logits, int dtype, size_t rows, int experts, int topk, int scoring, const void* bias, int groups, int group_topk,
              int renormalise, float scale, void* inds, void* scores, void* stream) {
     if (!logits || !inds || !scores) return T3_NULL_POINTER;

@@ -71,10 +71,20 @@ __device__ __forceinline__ uint32_t pack_as(float a, float b, int dt) {
 }
 
 // a whole warp's wait, in place
-template <bool CLUSTER>
 __device__ __forceinline__ void whole_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
-    fp8_wait_here<CLUSTER>(bar, parity, dead, err, bit);
+    fp8_wait_here<false, false>(bar, parity, dead, err, bit);
     __syncwarp();
+}
+// one behind the warp's last issue (see fp8_wait_here): a call in the split kernels, which have registers to spare for it (200 rows 7168 -> 576: 15.0 us
+// in place, 14.8 so; in the others it has the epilogue spill, 8192 rows 2048 -> 6144 135 -> 145)
+template <bool SPLIT, bool CLUSTER>
+__device__ __forceinline__ void last_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err, uint32_t bit) {
+    if (SPLIT) {
+        fp8_wait<CLUSTER>(bar, parity, dead, err, bit);
+    } else {
+        fp8_wait_here<CLUSTER, true>(bar, parity, dead, err, bit);
+        __syncwarp();
+    }
 }
 
 template <uint32_t N, bool SPLIT>
@@ -141,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     pdl_trigger();
                 }
                 const uint32_t s = rows_only ? i - ahead : slot, bar = full + 8u * s, at = base + s * kStageBytes;
-                if (!rows_only) whole_wait<false>(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
+                if (!rows_only) whole_wait(empty + 8u * s, parity, dead, a.err, kErrEmptyWait);
                 if (elect_one()) {
                     if (!rows_only) {
                         mbar_arrive_expect_tx_addr(bar, kStageBytes);
@@ -159,19 +169,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
             if (a.early && units == 0u) pdl_wait();
 #pragma unroll 1
             for (uint32_t i = 0; i < kStages; ++i) {  // the last products' arrivals are in before the CTA may end
-                whole_wait<false>(empty + 8u * slot, parity, dead, a.err, kErrEmptyWait);
+                last_wait<SPLIT, false>(empty + 8u * slot, parity, dead, a.err, kErrEmptyWait);
                 if (++slot == kStages) slot = 0, parity ^= 1u;
             }
         } else if (warp == kMmaWarp) {
             uint32_t slot = 0, parity = 0, acc = 0, acc_parity = 1;
+            uint32_t last = empty, last_parity = 1;  // of the last products' arrival
     #pragma unroll 1
             for (uint32_t t = first; t < tiles; t += stride) {
     #pragma unroll 1
                 for (uint32_t kb = k0; kb < k1; ++kb) {
                     const uint32_t at = base + slot * kStageBytes;
                     const uint64_t ad = umma_desc(at), bd = umma_desc(at + kRowBytes);
-                    whole_wait<false>(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
-                    whole_wait<false>(full + 8u * slot, parity, dead, a.err, kErrFullWait);
+                    whole_wait(acc_empty + 8u * acc, acc_parity, dead, a.err, kErrEmptyWait);
+                    whole_wait(full + 8u * slot, parity, dead, a.err, kErrFullWait);
                     tc_fence_after();
     #pragma unroll
                     for (uint32_t j = 0; j < 4u; ++j)  // 32 inputs each
@@ -181,11 +192,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                         umma_commit(acc_full + 8u * acc);
                     }
                     __syncwarp();
+                    last = empty + 8u * slot, last_parity = parity;
                     if (++slot == kStages) slot = 0, parity ^= 1u;
                     acc ^= 1u;
                     if (acc == 0u) acc_parity ^= 1u;
                 }
             }
+            last_wait<SPLIT, false>(last, last_parity, dead, a.err, kErrMmaWait);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
@@ -212,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
                     if (kb + p >= k1) break;
                     const float c = sx[p] * sw[p];
                     if (kb + p + 2u < k1) sx[p] = xs[kb + p + 2u], sw[p] = ws[kb + p + 2u];
-                    whole_wait<false>(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
+                    whole_wait(acc_full + 8u * acc, parity, dead, a.err, kErrMmaWait);
                     tc_fence_after();
                     const uint32_t from = tmem + acc * N + half * kMine + ((quarter * 32u) << 16);
                     // (the next sixteen columns on their way under the multiply-adds of these: 125 -> 115 us at 8192 rows 2048 -> 6144)
@@ -287,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm(const __grid_constant__ 
     }
     if (SPLIT) {
         // (a CTA arrives once all that was sent to it is there: past the barrier no copy reads from a CTA any more, nor writes to one)
-        whole_wait<true>(recv, 0, dead, a.err, kErrFullWait);
+        last_wait<true, true>(recv, 0, dead, a.err, kErrFullWait);
         __syncwarp();
         cluster_arrive_relaxed();
         if (a.early) pdl_wait();

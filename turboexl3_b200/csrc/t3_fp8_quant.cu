@@ -66,7 +66,27 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize(const void* x, size_t g
     }
 }
 
+// A warp waits twice for phases that nothing completes, as the kernels' roles do behind what they have issued: the first wait runs out and says so, the
+// second finds `dead` and takes no time.
+__global__ void fp8_wait_runs_out(uint32_t* err) {
+    __shared__ uint64_t bar[2];
+    __shared__ uint32_t dead;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar[0], 1u), mbar_init(&bar[1], 1u);
+        mbar_init_fence();
+        dead = 0u;
+    }
+    __syncthreads();
+    fp8_wait(smem_addr(&bar[0]), 0u, &dead, err, kErrMmaWait);
+    fp8_wait(smem_addr(&bar[1]), 0u, &dead, err, kErrFullWait);
+}
+
 }  // namespace
+
+cudaError_t launch_fp8_wait_runs_out(uint32_t* err, cudaStream_t stream) {
+    fp8_wait_runs_out<<<1, 32, 0, stream>>>(err);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_fp8_quantize(const void* x, int dt, size_t rows, uint32_t in, uint8_t* q, float* scale, bool overlap, cudaStream_t stream) {
     const size_t groups = rows * (in / 128u), per = kThreads / 16u;

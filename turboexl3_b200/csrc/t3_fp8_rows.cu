@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
     } else if (warp == kMmaWarp) {
         Slot s, c;
         uint32_t k = 0;  // gate|up, QUANT: the block's place in the slice, each twice
+        uint32_t last = bars + kBarEmpty, last_parity = 1;  // of the last products' arrival
 #pragma unroll 1
         for (uint32_t i = 0; i < blocks; ++i) {
             const uint32_t at = base + s.i * kStageBytes;
@@ -362,8 +363,10 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_rows(const __grid_constant__ 
                 umma_commit(bars + kBarAccFull + 8u * c.i);
             }
             __syncwarp();
+            last = bars + kBarEmpty + 8u * s.i, last_parity = s.parity;
             s.next(a.stages), c.next(kAcc);
         }
+        fp8_wait(last, last_parity, dead, a.err, kErrMmaWait);
     } else if (warp >= kScaleWarp) {
         // The columns' scales of one four's units, a lane a column. What lies in memory (the block's scale; the rows', where they came quantised)
         // is on its way to shared memory kAhead units before its use.
