@@ -4,9 +4,10 @@
 // among equals": keys are the picks' bit patterns made to order as whole numbers, so a round is two warp reductions and a look
 // through each lane's values. Without bias or groups the pick is the logit itself (both scorings rise with it); with them it is score + bias,
 // where two sums that differ in the last bits must still order as their exact values do: they are taken in 32 bits, and those that
-// a choice hangs on and that are too near each other once more in 64. (All rows in 64 bits: 27.5 us at 8192 rows of 256 experts.) Bound by
-// instructions on long prompts (1660 a row of 256 experts in 8 groups, 18.7 us at 8192 rows; 40 % of them the rounds), by latency on decode rows
-// (4.7 us at one row of 512, ten rounds).
+// a choice hangs on and that are too near each other once more in 64. (All rows in 64 bits: 27.5 us at 8192 rows of 256 experts.) Long prompts: 1670
+// instructions a row of 256 experts in 8 groups, 17.9 us at 8192 rows; a round is 69 of them, eight a third. While a multiprocessor has warps (31 of
+// 64 on average) its schedulers issue in 62 % of the cycles and wait for a warp's last instruction in the others; the grid is 1.4 rounds of CTAs, so over the
+// launch it is about half. Decode rows are bound by latency (4.8 us at one row of 512, ten rounds).
 #include <cfloat>
 
 #include "t3_fp8.cuh"
