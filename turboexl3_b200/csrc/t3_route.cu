@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
         if (a.groups > 1u) {
             __syncwarp();
             // a group's rank is by the sum of its two largest picks that are not removed: of those in shared memory the removed ones are -inf, and the
-            // live ones of -inf are looked for only where the row has one
+            // live ones of -inf are looked for only where the row has one and a group is short of two others
             const uint32_t g = lane / lanes;
             float first = -INFINITY, second = -INFINITY;
             if (g < a.groups) {
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32u) route_rows(const __grid_constant
                 first = fmaxf(first, f);
             }
             bool lowest_live = false;
-            if (odd) {
+            if (odd && __any_sync(kFull, g < a.groups && second == -INFINITY)) {
                 if (g < a.groups)
 #pragma unroll 1
                     for (uint32_t i = lane & (lanes - 1u); i < wide; i += lanes)
